@@ -480,6 +480,132 @@ int msc_slab_res_block(msc_slab_t s, const float* norm_w, const float* norm_b, c
  * its handling of a neighbour that never arrives without a second GPU. */
 int msc_wait_probe(msc_ctx_t ctx, int64_t budget_us, void* stream);
 
+/* ------------------------------------------ gated feed-forward blocks
+ * The residual block that mixes the channels of each row (voxel or token) on
+ * its own, beside the convolutional res_block: norm -> gated feed-forward ->
+ * [norm] -> gate and residual scale, with the backward pass of each part.  No
+ * counterpart in the reference's sparse path (its blocks are convolutions);
+ * norms, rows and sample indices are laid out as everywhere above.  Sizes:
+ * channels and hidden a multiple of 8, channels <= 8192, hidden <= 65536. */
+
+/* norm kinds: LayerNorm (v - mean) / sqrt(var + eps), RMSNorm
+ * v / sqrt(mean(v^2) + eps), over a row's channels */
+#define MSC_NORM_NONE 0
+#define MSC_NORM_LAYER 1
+#define MSC_NORM_RMS 2
+
+typedef struct {
+    int kind;
+    const float* w; /* [c] (NULL: ones) */
+    const float* b; /* [c] (NULL: zeros) */
+    float eps;
+} msc_norm;
+
+/* Norms before and after a block, fused with its gate and residual scale:
+ *   t = post(f);  r = res_scale * x + gate * t;  h = pre(r)
+ * x, r: the residual stream; f: the block's output; h: the next block's
+ * input, normalised from the unrounded r. */
+typedef struct {
+    int c;
+    int x_dtype;       /* residual stream: MSC_F32 or f_dtype */
+    int f_dtype;       /* branch (f and h) */
+    msc_norm post;
+    msc_norm pre;
+    const float* gate; /* NULL: ones; nsamples = 0: [c]; else [nsamples][c] */
+    int nsamples;      /* a row's sample is coords[i][3] (only read with a gate per sample) */
+    float res_scale;
+} msc_residual_norm_desc;
+
+/* One pass over n rows.  f may be NULL (r = res_scale * x: a stack's entry
+ * norm); r or h may be NULL where it is not wanted (with pre.kind
+ * MSC_NORM_NONE, h is r in the branch's type); r may be x and h may be f.  A
+ * sample index outside [0, nsamples) sets MSC_DEV_BAD_COORD (msc_check) and
+ * leaves that row's branch out. */
+int msc_residual_norm(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t n, const void* x, const void* f,
+                      const int32_t* coords, void* r, void* h, void* stream);
+
+/* Gradients; NULL members are not written. */
+typedef struct {
+    void* dx;      /* [n][c], x_dtype; may be dr */
+    void* df;      /* [n][c], f_dtype; may be dh */
+    float* gate;   /* as the gate: [c] or [nsamples][c] */
+    float* post_w; /* [c] */
+    float* post_b;
+    float* pre_w;
+    float* pre_b;
+} msc_residual_norm_grads;
+
+size_t msc_residual_norm_backward_workspace_bytes(int64_t n, int c, int nsamples);
+
+/* Backward pass of msc_residual_norm: r is the forward's output, dr and dh
+ * the gradients of r and h (one of them may be NULL: zero).  The norms'
+ * statistics are computed again from r and f.  Column sums are fp32 within a
+ * run of rows and double across them, in a fixed order (no atomics). */
+int msc_residual_norm_backward(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t n, const void* r,
+                               const void* f, const int32_t* coords, const void* dr, const void* dh,
+                               const msc_residual_norm_grads* grads, void* ws, size_t ws_bytes, void* stream);
+
+/* activations of the gate projection: x sigmoid(x); GELU in its tanh form;
+ * GELU with erf */
+#define MSC_ACT_SILU 0
+#define MSC_ACT_GELU 1
+#define MSC_ACT_GELU_ERF 2
+
+/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down */
+typedef struct {
+    int dtype;          /* x, y and the weights: MSC_F16 or MSC_BF16 */
+    int hidden;
+    int act;
+    const void* w_gate; /* [hidden][c] */
+    const void* w_up;   /* [hidden][c] */
+    const void* w_down; /* [c][hidden] */
+    const float* b_gate; /* [hidden] (may be NULL) */
+    const float* b_up;
+    const float* b_down; /* [c] (may be NULL) */
+} msc_ffn;
+
+size_t msc_gated_ffn_workspace_bytes(int64_t n, int c, int hidden);
+
+/* Accumulation, activation and gating are fp32; the hidden values are
+ * rounded once to the features' type (the tensor cores' operand).  y may be
+ * x. */
+int msc_gated_ffn(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, void* y, void* ws,
+                  size_t ws_bytes, void* stream);
+
+/* Gradients; NULL members are not written (the three weights together). */
+typedef struct {
+    void* dx;      /* [n][c]; neither x nor dy */
+    void* w_gate;  /* as the weights, in their type */
+    void* w_up;
+    void* w_down;
+    float* b_gate; /* as the biases, whether the block has them or not */
+    float* b_up;
+    float* b_down;
+} msc_ffn_grads;
+
+size_t msc_gated_ffn_backward_workspace_bytes(int64_t n, int c, int hidden);
+
+/* Backward pass of msc_gated_ffn from x and dy; the hidden values are
+ * computed again.  Sums over the rows run in a fixed order (no atomics). */
+int msc_gated_ffn_backward(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, const void* dy,
+                           const msc_ffn_grads* grads, void* ws, size_t ws_bytes, void* stream);
+
+/* One residual feed-forward block: x <- res_scale * x + gate * post(ffn(pre(x))). */
+typedef struct {
+    msc_ffn ffn;
+    msc_norm pre;
+    msc_norm post;
+    const float* gate; /* as in msc_residual_norm_desc, nsamples from the call */
+    float res_scale;
+} msc_ffn_block;
+
+/* nblocks residual feed-forward blocks in a row, in place on x (a level's
+ * block loop in one call, beside msc_res_stack): each block's exit and the
+ * next block's entry norm are one pass.  Workspace: of the largest hidden. */
+size_t msc_ffn_stack_workspace_bytes(int64_t n, int c, int hidden);
+int msc_ffn_stack(msc_ctx_t ctx, void* x, int x_dtype, int64_t n, int c, const int32_t* coords, int nsamples,
+                  int nblocks, const msc_ffn_block* blocks, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------ tracing */
 
 typedef struct {

@@ -4,9 +4,11 @@
 // every call runs inside guard(), which converts exceptions into a negative
 // status and a thread-local message; nothing throws across the boundary.
 #include "conv.h"
+#include "ffn.h"
 #include "gn.h"
 #include "ops.h"
 #include "plan.h"
+#include "rownorm.h"
 #include "topology.h"
 
 #include "../../include/moge_sparse_cuda.h"
@@ -954,6 +956,259 @@ int msc_nearest_up(msc_ctx_t ctx, const void* x, int x_dtype, int64_t np, int c,
         cuda_ok(msc::launch_gather_rows(t, np, b.cout, up_rows, nfine, skip, skip_dtype, y, y_dtype, ctx->status,
                                         S(stream)),
                 "up gather");
+    });
+}
+
+namespace {
+msc::NormParams norm_params(const msc_norm& m, const char* what) {
+    if (m.kind != MSC_NORM_NONE && m.kind != MSC_NORM_LAYER && m.kind != MSC_NORM_RMS)
+        fail(MSC_E_INVALID, std::string("unknown norm kind for ") + what);
+    if (m.kind == MSC_NORM_NONE) return msc::NormParams{msc::NORM_NONE, nullptr, nullptr, 1.0f};
+    if (!(m.eps > 0.0f)) fail(MSC_E_INVALID, std::string(what) + " norm eps must be positive");
+    need_aligned(m.w, 16, "norm weight");
+    need_aligned(m.b, 16, "norm bias");
+    return msc::NormParams{m.kind == MSC_NORM_LAYER ? msc::NORM_LAYER : msc::NORM_RMS, m.w, m.b, m.eps};
+}
+
+void need_rows(int64_t n) { need(n >= 0 && n < (int64_t(1) << 31) / 27, "row count out of range"); }
+
+// The checks shared by the residual norm and its backward pass.
+// Without a branch the post norm and the gate have nothing to act on.
+msc::RowNormArgs rownorm_args(msc_ctx_t ctx, const msc_residual_norm_desc* d, int64_t n, const int32_t* coords,
+                              bool branch) {
+    need(d != nullptr, "null residual norm descriptor");
+    need_dtype(d->x_dtype, "x");
+    need_dtype(d->f_dtype, "f");
+    if (!msc::rownorm_dtypes_supported(d->x_dtype, d->f_dtype))
+        fail(MSC_E_UNSUPPORTED, "the residual stream is fp32 or of the branch's type");
+    need_rows(n);
+    need(d->c > 0, "bad channel count");
+    if (d->c % 8 != 0 || d->c > msc::kRowNormMaxC)
+        fail(MSC_E_UNSUPPORTED, "channels must be a multiple of 8, at most " + std::to_string(msc::kRowNormMaxC));
+    msc::RowNormArgs a{};
+    a.n = n;
+    a.c = d->c;
+    a.x_dtype = d->x_dtype;
+    a.f_dtype = d->f_dtype;
+    a.post = norm_params(d->post, "post");
+    a.pre = norm_params(d->pre, "pre");
+    if (!branch) a.post.kind = msc::NORM_NONE;
+    a.gate = branch ? d->gate : nullptr;
+    need_aligned(a.gate, 16, "gate");
+    if (a.gate) {
+        need(d->nsamples >= 0 && d->nsamples <= (1 << 20), "nsamples out of range");
+        a.nsamples = d->nsamples;
+        if (d->nsamples) {
+            need(coords != nullptr || n == 0, "a gate per sample needs the coordinates");
+            need_aligned(coords, 16, "coords");
+            a.coords = coords;
+        }
+    }
+    a.res_scale = d->res_scale;
+    a.status = ctx->status;
+    return a;
+}
+
+void run_rownorm(msc_ctx_t ctx, msc::RowNormArgs a, const void* x, const void* f, void* r, void* h, cudaStream_t st) {
+    a.x = x;
+    a.f = f;
+    a.r = r;
+    a.h = h;
+    ProfScope ps(ctx, "residual_norm", st);
+    cuda_ok(msc::launch_rownorm(a, st), "residual norm launch");
+}
+
+struct FfnCall {
+    msc::FfnShape s;
+    msc::FfnWeights w;
+};
+FfnCall ffn_call(const msc_ffn* f, int64_t n, int c) {
+    need(f != nullptr, "null feed-forward block");
+    need_dtype(f->dtype, "the feed-forward block");
+    if (f->dtype == MSC_F32) fail(MSC_E_UNSUPPORTED, "feed-forward blocks are built for fp16 and bf16");
+    need(f->act == MSC_ACT_SILU || f->act == MSC_ACT_GELU || f->act == MSC_ACT_GELU_ERF, "unknown activation");
+    need_rows(n);
+    need(c > 0 && f->hidden > 0, "bad channel counts");
+    if (c % 8 != 0 || c > 8192 || f->hidden % 8 != 0 || f->hidden > 65536)
+        fail(MSC_E_UNSUPPORTED, "channels (at most 8192) and hidden size (at most 65536) must be multiples of 8");
+    need(f->w_gate && f->w_up && f->w_down, "null weights");
+    need_aligned(f->w_gate, 16, "w_gate");
+    need_aligned(f->w_up, 16, "w_up");
+    need_aligned(f->w_down, 16, "w_down");
+    need_aligned(f->b_gate, 16, "b_gate");
+    need_aligned(f->b_up, 16, "b_up");
+    need_aligned(f->b_down, 16, "b_down");
+    FfnCall k{};
+    k.s = msc::FfnShape{n, c, f->hidden, f->dtype,
+                        f->act == MSC_ACT_SILU ? msc::ACT_SILU : (f->act == MSC_ACT_GELU ? msc::ACT_GELU : msc::ACT_GELU_ERF)};
+    k.w = msc::FfnWeights{f->w_gate, f->w_up, f->w_down, f->b_gate, f->b_up, f->b_down};
+    return k;
+}
+
+bool ffn_sizes_ok(int64_t n, int c, int hidden) {
+    return n >= 0 && n < (int64_t(1) << 31) / 27 && c > 0 && c <= 8192 && hidden > 0 && hidden <= 65536;
+}
+}  // namespace
+
+int msc_residual_norm(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t n, const void* x, const void* f,
+                      const int32_t* coords, void* r, void* h, void* stream) {
+    return guard([&] {
+        need_ctx(ctx);
+        const auto a = rownorm_args(ctx, desc, n, coords, f != nullptr);
+        if (n == 0) return;
+        need(x && (r || h), "null pointer");
+        need(a.pre.kind == msc::NORM_NONE || h, "a pre norm needs its output");
+        need_aligned(x, 16, "x");
+        need_aligned(f, 16, "f");
+        need_aligned(r, 16, "r");
+        need_aligned(h, 16, "h");
+        run_rownorm(ctx, a, x, f, r, h, S(stream));
+    });
+}
+
+size_t msc_residual_norm_backward_workspace_bytes(int64_t n, int c, int nsamples) {
+    if (n < 0 || c <= 0 || c > msc::kRowNormMaxC || nsamples < 0 || nsamples > (1 << 20)) return 0;
+    return align256(msc::rownorm_backward_workspace_bytes(n, c, nsamples));
+}
+
+int msc_residual_norm_backward(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t n, const void* r,
+                               const void* f, const int32_t* coords, const void* dr, const void* dh,
+                               const msc_residual_norm_grads* grads, void* ws, size_t ws_bytes, void* stream) {
+    return guard([&] {
+        need_ctx(ctx);
+        auto a = rownorm_args(ctx, desc, n, coords, f != nullptr || n == 0);
+        need(grads != nullptr, "null gradients");
+        need(ws != nullptr, "null workspace");
+        if (n > 0) {
+            need(dr || dh, "no gradient to propagate");
+            need(a.pre.kind == msc::NORM_NONE || (r && dh), "the pre norm's backward pass needs r and dh");
+        }
+        need_aligned(r, 16, "r");
+        need_aligned(f, 16, "f");
+        need_aligned(dr, 16, "dr");
+        need_aligned(dh, 16, "dh");
+        need_aligned(grads->dx, 16, "dx");
+        need_aligned(grads->df, 16, "df");
+        need_aligned(ws, 256, "workspace");
+        need_ws(ws_bytes, msc::rownorm_backward_workspace_bytes(n, a.c, a.nsamples));
+        need(f || n == 0 || !grads->df, "gradient of a branch that is absent");
+        need(a.gate || !grads->gate, "gradient of a gate that is absent");
+        need(a.post.kind != msc::NORM_NONE || (!grads->post_w && !grads->post_b), "gradient of a post norm that is absent");
+        need(a.pre.kind != msc::NORM_NONE || (!grads->pre_w && !grads->pre_b), "gradient of a pre norm that is absent");
+        a.x = r;
+        a.f = f;
+        a.dr = dr;
+        a.dh = dh;
+        a.dx = grads->dx;
+        a.df = grads->df;
+        const msc::RowNormGrads g{grads->gate, grads->post_w, grads->post_b, grads->pre_w, grads->pre_b};
+        ProfScope ps(ctx, "residual_norm_backward", S(stream));
+        cuda_ok(msc::launch_rownorm_backward(a, g, ws, S(stream)), "residual norm backward launch");
+    });
+}
+
+size_t msc_gated_ffn_workspace_bytes(int64_t n, int c, int hidden) {
+    return ffn_sizes_ok(n, c, hidden) ? align256(msc::ffn_workspace_bytes(n, c, hidden)) : 0;
+}
+
+int msc_gated_ffn(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, void* y, void* ws,
+                  size_t ws_bytes, void* stream) {
+    return guard([&] {
+        need_ctx(ctx);
+        const FfnCall k = ffn_call(ffn, n, c);
+        if (n == 0) return;
+        need(x && y && ws, "null pointer");
+        need_aligned(x, 16, "x");
+        need_aligned(y, 16, "y");
+        need_aligned(ws, 256, "workspace");
+        need_ws(ws_bytes, msc::ffn_workspace_bytes(n, c, ffn->hidden));
+        ProfScope ps(ctx, "gated_ffn", S(stream));
+        cuda_ok(msc::launch_ffn(k.s, x, k.w, y, ws, ctx->status, S(stream)), "gated ffn launch");
+    });
+}
+
+size_t msc_gated_ffn_backward_workspace_bytes(int64_t n, int c, int hidden) {
+    return ffn_sizes_ok(n, c, hidden) ? align256(msc::ffn_backward_workspace_bytes(n, c, hidden)) : 0;
+}
+
+int msc_gated_ffn_backward(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, const void* dy,
+                           const msc_ffn_grads* grads, void* ws, size_t ws_bytes, void* stream) {
+    return guard([&] {
+        need_ctx(ctx);
+        const FfnCall k = ffn_call(ffn, n, c);
+        need(grads != nullptr, "null gradients");
+        const bool w_any = grads->w_gate || grads->w_up || grads->w_down;
+        need(!w_any || (grads->w_gate && grads->w_up && grads->w_down),
+             "the weight gradients are asked for together or not at all");
+        need(grads->dx || w_any || grads->b_gate || grads->b_up || grads->b_down, "no gradient asked for");
+        need_aligned(grads->dx, 16, "dx");
+        need_aligned(grads->w_gate, 16, "w_gate gradient");
+        need_aligned(grads->w_up, 16, "w_up gradient");
+        need_aligned(grads->w_down, 16, "w_down gradient");
+        if (n > 0) {
+            need(x && dy && ws, "null pointer");
+            need(!grads->dx || (grads->dx != x && grads->dx != dy), "dx must not be x or dy: the weight gradients read them later");
+            need_aligned(x, 16, "x");
+            need_aligned(dy, 16, "dy");
+            need_aligned(ws, 256, "workspace");
+            need_ws(ws_bytes, msc::ffn_backward_workspace_bytes(n, c, ffn->hidden));
+        }
+        const msc::FfnGrads g{grads->dx, grads->w_gate, grads->w_up, grads->w_down,
+                              grads->b_gate, grads->b_up, grads->b_down};
+        ProfScope ps(ctx, "gated_ffn_backward", S(stream));
+        cuda_ok(msc::launch_ffn_backward(k.s, x, dy, k.w, g, ws, ctx->status, S(stream)), "gated ffn backward launch");
+    });
+}
+
+size_t msc_ffn_stack_workspace_bytes(int64_t n, int c, int hidden) {
+    if (!ffn_sizes_ok(n, c, hidden)) return 0;
+    return 2 * align256(static_cast<size_t>(n) * c * 2) + align256(msc::ffn_workspace_bytes(n, c, hidden));
+}
+
+int msc_ffn_stack(msc_ctx_t ctx, void* x, int x_dtype, int64_t n, int c, const int32_t* coords, int nsamples,
+                  int nblocks, const msc_ffn_block* blocks, void* ws, size_t ws_bytes, void* stream) {
+    return guard([&] {
+        need_ctx(ctx);
+        need(nblocks >= 0, "negative block count");
+        if (nblocks == 0) return;
+        need(blocks != nullptr, "null blocks");
+        size_t want = 0;
+        // every block is checked before the first launch: a refused stack
+        // leaves x as it was
+        for (int i = 0; i < nblocks; ++i) {
+            ffn_call(&blocks[i].ffn, n, c);
+            need(blocks[i].ffn.dtype == blocks[0].ffn.dtype, "the blocks of a stack share one type");
+            const msc_residual_norm_desc d{c, x_dtype, blocks[i].ffn.dtype, blocks[i].post, blocks[i].pre,
+                                           blocks[i].gate, nsamples, blocks[i].res_scale};
+            rownorm_args(ctx, &d, n, coords, true);
+            want = std::max(want, msc_ffn_stack_workspace_bytes(n, c, blocks[i].ffn.hidden));
+        }
+        if (n == 0) return;
+        need(x && ws, "null pointer");
+        need_aligned(x, 16, "x");
+        need_aligned(ws, 256, "workspace");
+        need_ws(ws_bytes, want);
+        const size_t row_bytes = align256(static_cast<size_t>(n) * c * 2);
+        char* h = static_cast<char*>(ws);
+        char* f = h + row_bytes;
+        char* scratch = f + row_bytes;
+        const int dt = blocks[0].ffn.dtype;
+        // a block's exit (post norm, gate, residual scale) and the next
+        // block's entry norm are one pass
+        const msc_norm none{MSC_NORM_NONE, nullptr, nullptr, 0.0f};
+        const msc_residual_norm_desc entry{c, x_dtype, dt, none, blocks[0].pre, nullptr, 0, 1.0f};
+        run_rownorm(ctx, rownorm_args(ctx, &entry, n, nullptr, false), x, nullptr, nullptr, h, S(stream));
+        for (int i = 0; i < nblocks; ++i) {
+            const FfnCall k = ffn_call(&blocks[i].ffn, n, c);
+            {
+                ProfScope ps(ctx, "gated_ffn", S(stream));
+                cuda_ok(msc::launch_ffn(k.s, h, k.w, f, scratch, ctx->status, S(stream)), "gated ffn launch");
+            }
+            const bool last = i + 1 == nblocks;
+            const msc_residual_norm_desc d{c, x_dtype, dt, blocks[i].post, last ? none : blocks[i + 1].pre,
+                                           blocks[i].gate, nsamples, blocks[i].res_scale};
+            run_rownorm(ctx, rownorm_args(ctx, &d, n, coords, true), x, f, x, last ? nullptr : h, S(stream));
+        }
     });
 }
 

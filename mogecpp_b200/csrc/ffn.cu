@@ -1,0 +1,460 @@
+// Gated feed-forward block over the channels of each row, [n][c] rows of fp16
+// or bf16:
+//   g = x Wg^T + bg;  u = x Wu^T + bu;  h = act(g) * u;  y = h Wd^T + bd
+// (SwiGLU / GeGLU), and its backward pass, which computes g and u again:
+//   dh = dy Wd;  dg = dh u act'(g);  du = dh act(g)
+//   dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x;  dWd = dy^T h
+//   dbg, dbu, dbd = column sums of dg, du, dy
+//
+// Every product runs on tcgen05 (ffn_gemm.cuh) with fp32 accumulators; the
+// activation, its derivative and the gating product are fp32 in the epilogue.
+// h, dg and du are rounded once to the features' type, because the tensor
+// cores take them as 16-bit operands of the next product; the bias sums are
+// taken from the unrounded fp32 values.
+#include "ffn.h"
+
+#include "conv.h"
+#include "ffn_gemm.cuh"
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+namespace msc {
+namespace {
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static std::mutex mu;
+    static EncodeTiled fn = nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(p);
+    }
+    return fn;
+}
+
+constexpr int kSms = 148;  // B200; fixed, so that the split of a sum and the workspace do not depend on the device
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Column tile of a product with `cols` output columns: the widest that still
+// gives every SM a tile (wider tiles read less shared memory per product;
+// narrower ones spread few rows over more SMs).
+int col_tile(int64_t m_tiles, int cols) {
+    for (int ht = 256; ht > 64; ht /= 2)
+        if (cols > ht / 2 && m_tiles * cdiv(cols, ht) >= kSms) return ht;
+    return 64;
+}
+
+// Splits of a K of `ksteps` steps when `tiles` output tiles leave SMs idle.
+int k_splits(int64_t tiles, int ksteps, int min_steps, int* ksplit) {
+    int64_t s = tiles > 0 && tiles * 2 <= kSms ? kSms / tiles : 1;
+    s = std::max<int64_t>(1, std::min<int64_t>(s, ksteps / min_steps));
+    ksteps = std::max(ksteps, 1);
+    *ksplit = static_cast<int>(cdiv(ksteps, s));
+    return static_cast<int>(cdiv(ksteps, *ksplit));
+}
+
+struct ProjPlan {
+    int ht, splits, ksplit;
+};
+ProjPlan proj_plan(int64_t n, int cols, int ksteps) {
+    ProjPlan p{};
+    const int64_t m = cdiv(n, 128);
+    p.ht = col_tile(m, cols);
+    p.splits = k_splits(m * cdiv(cols, p.ht), ksteps, 4, &p.ksplit);
+    return p;
+}
+
+struct DwPlan {
+    int ht, splits, ksplit, tiles;
+};
+DwPlan dw_plan(int64_t n, int c, int hidden) {
+    DwPlan p{};
+    p.ht = c > 128 ? 256 : (c > 64 ? 128 : 64);
+    p.tiles = static_cast<int>(2 * cdiv(hidden, 128) * cdiv(c, p.ht) + cdiv(c, 128) * cdiv(hidden, p.ht));
+    const int ksteps = static_cast<int>(cdiv(n, 64));
+    p.splits = k_splits(p.tiles, ksteps, 4, &p.ksplit);
+    // no sum in one accumulator runs over more than 32768 rows: the tensor
+    // core's fp32 accumulator truncates, a drift that grows with the chain
+    if (p.ksplit > 512) {
+        p.ksplit = 512;
+        p.splits = static_cast<int>(cdiv(ksteps, p.ksplit));
+    }
+    return p;
+}
+
+template <int MODE, int HT>
+cudaError_t launch_gemm_t(const FfnGemmArgs& a, cudaStream_t st) {
+    using C = FfnCfg<MODE, HT>;
+    auto kern = ffn_gemm_kernel<MODE, HT>;
+    static std::mutex mu;
+    static int num_sms[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    int sms = 0;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!num_sms[dev]) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            if (e != cudaSuccess) return e;
+            int count = 0;
+            e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+            if (e != cudaSuccess) return e;
+            num_sms[dev] = count;
+        }
+        sms = num_sms[dev];
+    }
+    const int total = a.tiles * a.splits;
+    kern<<<std::min(total, sms), kFfnThreads, C::SMEM, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <int MODE>
+cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, cudaStream_t st) {
+    if constexpr (MODE == FFN_HBACK) return launch_gemm_t<MODE, 64>(a, st);
+    if constexpr (MODE == FFN_HIDDEN) {
+        if (ht == 128) return launch_gemm_t<MODE, 128>(a, st);
+        return launch_gemm_t<MODE, 64>(a, st);
+    }
+    if constexpr (MODE == FFN_PROJ || MODE == FFN_DX || MODE == FFN_DW) {
+        if (ht == 256) return launch_gemm_t<MODE, 256>(a, st);
+        if (ht == 128) return launch_gemm_t<MODE, 128>(a, st);
+        return launch_gemm_t<MODE, 64>(a, st);
+    }
+    return cudaErrorInvalidValue;
+}
+
+void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht) {
+    a.nprob = 1;
+    a.m_tiles[0] = static_cast<int>(cdiv(rows, 128));
+    a.n_tiles[0] = static_cast<int>(cdiv(cols, ht));
+    a.rows[0] = static_cast<int>(rows);
+    a.cols[0] = cols;
+    a.tiles = a.m_tiles[0] * a.n_tiles[0];
+    a.splits = 1;
+    a.ksplit = a.ksteps[0] + a.ksteps[1];
+}
+
+// out[i] = sum over the splits of part[s][i] (+ bias of column i % cols), in
+// split order; four elements a thread.
+struct SplitSumArgs {
+    const float* part;
+    int64_t stride;      // floats per split
+    int splits;
+    void* out[3];
+    int64_t begin[4];    // first element of each output, and the end
+    const float* bias;
+    int cols;
+    int bf16;
+};
+__global__ void __launch_bounds__(256) split_sum_kernel(const SplitSumArgs a) {
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    if (i >= a.begin[3]) return;
+    float4 s = *reinterpret_cast<const float4*>(a.part + i);
+    for (int k = 1; k < a.splits; ++k) {
+        const float4 t = *reinterpret_cast<const float4*>(a.part + k * a.stride + i);
+        s.x += t.x, s.y += t.y, s.z += t.z, s.w += t.w;
+    }
+    if (a.bias) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + i % a.cols));
+        s.x += b.x, s.y += b.y, s.z += b.z, s.w += b.w;
+    }
+    const int p = i >= a.begin[2] ? 2 : (i >= a.begin[1] ? 1 : 0);
+    uint2 w;
+    if (a.bf16) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+        const __half2 lo = __floats2half2_rn(s.x, s.y), hi = __floats2half2_rn(s.z, s.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out[p]) + (i - a.begin[p])) = w;
+}
+
+cudaError_t launch_split_sum(const SplitSumArgs& a, cudaStream_t st) {
+    split_sum_kernel<<<static_cast<unsigned>(cdiv(a.begin[3], 1024)), 256, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+// Column sums of a 16-bit [n][c] matrix over a run of rows per block, fp32.
+constexpr int kColsumRows = 256;
+__global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, float* part) {
+    // 32 threads x 8 columns, 8 rows in flight
+    __shared__ float red[8][32][9];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int col = (blockIdx.y * 32 + tx) * 8;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kColsumRows;
+    const int64_t r1 = min(r0 + kColsumRows, n);
+    float s[8] = {};
+    if (col < c)
+        for (int64_t r = r0 + ty; r < r1; r += 8) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(y) + r * c + col);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 t = bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
+                                      : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                s[2 * e] += t.x, s[2 * e + 1] += t.y;
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[ty][tx][e] = s[e];
+    __syncthreads();
+    if (ty == 0 && col < c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float q = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) q += red[w][tx][e];
+            part[static_cast<int64_t>(blockIdx.x) * c + col + e] = q;
+        }
+    }
+}
+
+// Totals over the units of part [units][cols] in double and in a fixed order;
+// the first n0 columns go to out0, the others to out1 (either may be NULL).
+__global__ void __launch_bounds__(1024) column_total_kernel(const float* part, int64_t units, int cols, int n0,
+                                                            float* out0, float* out1) {
+    __shared__ double red[32][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    double s = 0.0;
+    if (col < cols)
+        for (int64_t u = threadIdx.y; u < units; u += 32) s += part[u * cols + col];
+    red[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 16; o >= 1; o >>= 1) {
+        if (threadIdx.y < o) red[threadIdx.y][threadIdx.x] += red[threadIdx.y + o][threadIdx.x];
+        __syncthreads();
+    }
+    if (threadIdx.y == 0 && col < cols) {
+        float* o = col < n0 ? out0 : out1;
+        if (o) o[col < n0 ? col : col - n0] = static_cast<float>(red[0][threadIdx.x]);
+    }
+}
+
+cudaError_t launch_column_total(const float* part, int64_t units, int cols, int n0, float* out0, float* out1,
+                                cudaStream_t st) {
+    column_total_kernel<<<static_cast<unsigned>(cdiv(cols, 32)), dim3(32, 32), 0, st>>>(part, units, cols, n0, out0, out1);
+    return cudaGetLastError();
+}
+
+#define MSC_TRY(expr)                        \
+    do {                                     \
+        const cudaError_t e_ = (expr);       \
+        if (e_ != cudaSuccess) return e_;    \
+    } while (0)
+
+struct FwdWs {
+    size_t hidden, part, total;
+};
+FwdWs fwd_ws(int64_t n, int c, int hidden) {
+    FwdWs w{};
+    const ProjPlan p = proj_plan(n, c, static_cast<int>(cdiv(hidden, 64)));
+    w.hidden = 0;
+    w.part = align256(static_cast<size_t>(n) * hidden * 2);
+    w.total = w.part + (p.splits > 1 ? align256(static_cast<size_t>(p.splits) * n * c * 4) : 0);
+    return w;
+}
+
+struct BwdWs {
+    size_t dg, du, h, bias, dbd, part, total;
+};
+BwdWs bwd_ws(int64_t n, int c, int hidden) {
+    BwdWs w{};
+    const size_t nh = align256(static_cast<size_t>(n) * hidden * 2);
+    w.dg = 0;
+    w.du = nh;
+    w.h = 2 * nh;
+    w.bias = 3 * nh;
+    w.dbd = w.bias + align256(static_cast<size_t>(cdiv(n, 128)) * 2 * hidden * 4);
+    w.part = w.dbd + align256(static_cast<size_t>(cdiv(n, kColsumRows)) * c * 4);
+    const ProjPlan px = proj_plan(n, c, static_cast<int>(2 * cdiv(hidden, 64)));
+    const DwPlan pw = dw_plan(n, c, hidden);
+    size_t part = px.splits > 1 ? static_cast<size_t>(px.splits) * n * c * 4 : 0;
+    if (pw.splits > 1) part = std::max(part, static_cast<size_t>(pw.splits) * 3 * c * hidden * 4);
+    w.total = w.part + align256(part);
+    return w;
+}
+
+}  // namespace
+
+cudaError_t make_map_16bit(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int box_rows) {
+    const EncodeTiled enc = encode_tiled();
+    if (!enc) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t es[2] = {1, 1};
+    const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                           const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+size_t ffn_workspace_bytes(int64_t n, int c, int hidden) { return fwd_ws(n, c, hidden).total; }
+size_t ffn_backward_workspace_bytes(int64_t n, int c, int hidden) { return bwd_ws(n, c, hidden).total; }
+
+cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, void* y, void* ws, uint32_t* status,
+                       cudaStream_t st) {
+    if (s.n == 0) return cudaSuccess;
+    const bool bf = s.dtype == DT_BF16;
+    const FwdWs o = fwd_ws(s.n, s.c, s.hidden);
+    char* base = static_cast<char*>(ws);
+    void* h = base + o.hidden;
+    const int64_t m = cdiv(s.n, 128);
+    {
+        FfnGemmArgs a{};
+        const int ht = m * cdiv(s.hidden, 128) >= kSms ? 128 : 64;
+        MSC_TRY(make_map_16bit(&a.ma[0], x, bf, s.n, s.c, 128));
+        MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, ht));
+        MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, ht));
+        MSC_TRY(make_map_16bit(&a.mo[0], h, bf, s.n, s.hidden, 128));
+        a.ksteps[0] = static_cast<int>(cdiv(s.c, 64));
+        one_problem(a, s.n, s.hidden, ht);
+        a.bias0 = w.b_gate, a.bias1 = w.b_up;
+        a.act = s.act, a.bf16 = bf, a.status = status;
+        MSC_TRY(launch_gemm<FFN_HIDDEN>(a, ht, st));
+    }
+    FfnGemmArgs a{};
+    a.ksteps[0] = static_cast<int>(cdiv(s.hidden, 64));
+    const ProjPlan p = proj_plan(s.n, s.c, a.ksteps[0]);
+    MSC_TRY(make_map_16bit(&a.ma[0], h, bf, s.n, s.hidden, 128));
+    MSC_TRY(make_map_16bit(&a.mb[0], w.w_down, bf, s.c, s.hidden, p.ht));
+    MSC_TRY(make_map_16bit(&a.mo[0], y, bf, s.n, s.c, 128));
+    one_problem(a, s.n, s.c, p.ht);
+    a.splits = p.splits, a.ksplit = p.ksplit;
+    a.bias0 = w.b_down;
+    a.bf16 = bf, a.status = status;
+    if (p.splits > 1) {
+        a.partial = reinterpret_cast<float*>(base + o.part);
+        a.partial_split = s.n * s.c;
+    }
+    MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, st));
+    if (p.splits > 1) {
+        const int64_t e = s.n * s.c;
+        const SplitSumArgs r{a.partial, e, p.splits, {y, nullptr, nullptr}, {0, e, e, e}, w.b_down, s.c, bf};
+        MSC_TRY(launch_split_sum(r, st));
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy, const FfnWeights& w,
+                                const FfnGrads& g, void* ws, uint32_t* status, cudaStream_t st) {
+    const bool bf = s.dtype == DT_BF16;
+    const int64_t ch = static_cast<int64_t>(s.c) * s.hidden;
+    if (s.n == 0) {
+        if (g.w_gate) {
+            MSC_TRY(cudaMemsetAsync(g.w_gate, 0, ch * 2, st));
+            MSC_TRY(cudaMemsetAsync(g.w_up, 0, ch * 2, st));
+            MSC_TRY(cudaMemsetAsync(g.w_down, 0, ch * 2, st));
+        }
+        if (g.b_gate) MSC_TRY(cudaMemsetAsync(g.b_gate, 0, s.hidden * sizeof(float), st));
+        if (g.b_up) MSC_TRY(cudaMemsetAsync(g.b_up, 0, s.hidden * sizeof(float), st));
+        if (g.b_down) MSC_TRY(cudaMemsetAsync(g.b_down, 0, s.c * sizeof(float), st));
+        return cudaSuccess;
+    }
+    const BwdWs o = bwd_ws(s.n, s.c, s.hidden);
+    char* base = static_cast<char*>(ws);
+    void* dg = base + o.dg;
+    void* du = base + o.du;
+    void* h = base + o.h;
+    float* part = reinterpret_cast<float*>(base + o.part);
+    const int kc = static_cast<int>(cdiv(s.c, 64)), kh = static_cast<int>(cdiv(s.hidden, 64));
+    const int64_t m = cdiv(s.n, 128);
+    {
+        FfnGemmArgs a{};
+        MSC_TRY(make_map_16bit(&a.ma[0], x, bf, s.n, s.c, 128));
+        MSC_TRY(make_map_16bit(&a.ma[1], dy, bf, s.n, s.c, 128));
+        MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, 64));
+        MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, 64));
+        MSC_TRY(make_map_16bit(&a.mb[2], w.w_down, bf, s.c, s.hidden, 64));
+        MSC_TRY(make_map_16bit(&a.mo[0], dg, bf, s.n, s.hidden, 128));
+        MSC_TRY(make_map_16bit(&a.mo[1], du, bf, s.n, s.hidden, 128));
+        MSC_TRY(make_map_16bit(&a.mo[2], h, bf, s.n, s.hidden, 128));
+        a.ksteps[0] = a.ksteps[1] = kc;
+        one_problem(a, s.n, s.hidden, 64);
+        a.bias0 = w.b_gate, a.bias1 = w.b_up;
+        if (g.b_gate || g.b_up) a.bias_part = reinterpret_cast<float*>(base + o.bias);
+        a.act = s.act, a.bf16 = bf, a.status = status;
+        MSC_TRY(launch_gemm<FFN_HBACK>(a, 64, st));
+        if (a.bias_part) MSC_TRY(launch_column_total(a.bias_part, m, 2 * s.hidden, s.hidden, g.b_gate, g.b_up, st));
+    }
+    if (g.b_down) {
+        float* cp = reinterpret_cast<float*>(base + o.dbd);
+        const int64_t units = cdiv(s.n, kColsumRows);
+        colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 256))), 256, 0, st>>>(
+            dy, s.n, s.c, bf, cp);
+        MSC_TRY(cudaGetLastError());
+        MSC_TRY(launch_column_total(cp, units, s.c, s.c, g.b_down, nullptr, st));
+    }
+    if (g.dx) {
+        FfnGemmArgs a{};
+        const ProjPlan p = proj_plan(s.n, s.c, 2 * kh);
+        MSC_TRY(make_map_16bit(&a.ma[0], dg, bf, s.n, s.hidden, 128));
+        MSC_TRY(make_map_16bit(&a.ma[1], du, bf, s.n, s.hidden, 128));
+        MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, 64));
+        MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, 64));
+        MSC_TRY(make_map_16bit(&a.mo[0], g.dx, bf, s.n, s.c, 128));
+        a.ksteps[0] = a.ksteps[1] = kh;
+        one_problem(a, s.n, s.c, p.ht);
+        a.splits = p.splits, a.ksplit = p.ksplit;
+        a.bf16 = bf, a.status = status;
+        if (p.splits > 1) {
+            a.partial = part;
+            a.partial_split = s.n * s.c;
+        }
+        MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, st));
+        if (p.splits > 1) {
+            const int64_t e = s.n * s.c;
+            const SplitSumArgs r{part, e, p.splits, {g.dx, nullptr, nullptr}, {0, e, e, e}, nullptr, s.c, bf};
+            MSC_TRY(launch_split_sum(r, st));
+        }
+    }
+    if (g.w_gate) {
+        FfnGemmArgs a{};
+        const DwPlan p = dw_plan(s.n, s.c, s.hidden);
+        const void* am[3] = {dg, du, dy};
+        const void* bm[3] = {x, x, h};
+        void* om[3] = {g.w_gate, g.w_up, g.w_down};
+        a.nprob = 3;
+        for (int i = 0; i < 3; ++i) {
+            const int rows = i < 2 ? s.hidden : s.c, cols = i < 2 ? s.c : s.hidden;
+            MSC_TRY(make_map_16bit(&a.ma[i], am[i], bf, s.n, rows, 64));
+            MSC_TRY(make_map_16bit(&a.mb[i], bm[i], bf, s.n, cols, 64));
+            MSC_TRY(make_map_16bit(&a.mo[i], om[i], bf, rows, cols, 128));
+            a.m_tiles[i] = static_cast<int>(cdiv(rows, 128));
+            a.n_tiles[i] = static_cast<int>(cdiv(cols, p.ht));
+            a.rows[i] = rows, a.cols[i] = cols;
+            a.partial_prob[i] = i * ch;
+        }
+        a.tiles = p.tiles;
+        a.ksteps[0] = static_cast<int>(cdiv(s.n, 64));
+        a.splits = p.splits, a.ksplit = p.ksplit;
+        a.bf16 = bf, a.status = status;
+        if (p.splits > 1) {
+            a.partial = part;
+            a.partial_split = 3 * ch;
+        }
+        MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, st));
+        if (p.splits > 1) {
+            const SplitSumArgs r{part, 3 * ch, p.splits, {om[0], om[1], om[2]}, {0, ch, 2 * ch, 3 * ch}, nullptr, s.c, bf};
+            MSC_TRY(launch_split_sum(r, st));
+        }
+    }
+    return cudaSuccess;
+}
+
+}  // namespace msc

@@ -1,0 +1,61 @@
+// Tiled TMA copies (cp.async.bulk.tensor) and the tensor maps they take.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace msc {
+
+// Tile of a 2-D tensor map into shared memory, completing on an mbarrier.
+// x is the innermost coordinate and stays a multiple of 16 bytes.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Tile from shared memory to global memory (rows and columns past the
+// tensor's extents are not written), tracked by the thread's bulk groups.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
+                 "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// The thread's stores have read their shared memory / are complete.
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// Shared-memory matrix descriptor, MN-major, 128-byte swizzle: the tile lies
+// as [group of 64 MN][k][64 MN x 16 bit], i.e. 128-byte rows along MN, 8-row
+// groups of k 1024 B apart (stride byte offset), groups of 64 MN
+// group_bytes apart (leading byte offset).
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t smem_addr, uint32_t group_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3fffu);
+    d |= static_cast<uint64_t>((group_bytes >> 4) & 0x3fffu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// Instruction-descriptor bits of an MN-major A / B operand.
+constexpr uint32_t kIdescAMn = 1u << 15, kIdescBMn = 1u << 16;
+
+// 128B-swizzled tensor map of a row-major [rows][cols] matrix of 16-bit
+// elements (cols a multiple of 8, 16-byte aligned base) with boxes of 64
+// columns x box_rows rows; elements outside read as zero.
+cudaError_t make_map_16bit(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int64_t cols, int box_rows);
+
+}  // namespace msc

@@ -16,6 +16,9 @@ MSC_OK = 0
 MSC_F32, MSC_F16, MSC_BF16 = 0, 1, 2
 MSC_PLAN_TAP_ORDER = 0
 MSC_W_F32, MSC_W_F16, MSC_W_Q8_0 = 0, 1, 8
+MSC_E_INVALID = -1
+MSC_NORM_NONE, MSC_NORM_LAYER, MSC_NORM_RMS = 0, 1, 2
+MSC_ACT_SILU, MSC_ACT_GELU, MSC_ACT_GELU_ERF = 0, 1, 2
 DEV_TIMEOUT, DEV_HASH_FULL, DEV_BAD_COORD, DEV_DUP_COORD, DEV_POOL_OVERFLOW, DEV_BAD_INDEX = 1, 2, 4, 8, 16, 32
 
 _vp, _i64, _sz, _i32 = C.c_void_p, C.c_int64, C.c_size_t, C.c_int
@@ -83,6 +86,15 @@ SIGNATURES = {
     "msc_slab_features_ptr": (C.c_int, [_vp, C.POINTER(_vp)]),
     "msc_slab_res_block": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "msc_wait_probe": (C.c_int, [_vp, _i64, _vp]),
+    "msc_residual_norm": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "msc_residual_norm_backward_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "msc_residual_norm_backward": (C.c_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "msc_gated_ffn_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "msc_gated_ffn": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "msc_gated_ffn_backward_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "msc_gated_ffn_backward": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "msc_ffn_stack_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "msc_ffn_stack": (C.c_int, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _sz, _vp]),
     "msc_profile_enable": (C.c_int, [_vp, _i32]),
     "msc_profile_read": (C.c_int, [_vp, _vp, _i32, C.POINTER(_i32)]),
 }
@@ -108,6 +120,36 @@ class ConvFusion(C.Structure):
     """msc_conv_fusion: prologue (LayerNorm, SiLU) and epilogue (SiLU, residual) of a fused conv."""
     _fields_ = [("layer_norm", C.c_int), ("norm_w", C.c_void_p), ("norm_b", C.c_void_p), ("eps", C.c_float),
                 ("silu_in", C.c_int), ("silu_out", C.c_int), ("residual", C.c_void_p), ("residual_dtype", C.c_int)]
+
+
+class Norm(C.Structure):
+    """msc_norm: LayerNorm / RMSNorm over a row's channels."""
+    _fields_ = [("kind", C.c_int), ("w", C.c_void_p), ("b", C.c_void_p), ("eps", C.c_float)]
+
+
+class ResidualNormDesc(C.Structure):
+    """msc_residual_norm_desc: r = res_scale * x + gate * post(f), h = pre(r)."""
+    _fields_ = [("c", C.c_int), ("x_dtype", C.c_int), ("f_dtype", C.c_int), ("post", Norm), ("pre", Norm),
+                ("gate", C.c_void_p), ("nsamples", C.c_int), ("res_scale", C.c_float)]
+
+
+class ResidualNormGrads(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("dx", "df", "gate", "post_w", "post_b", "pre_w", "pre_b")]
+
+
+class Ffn(C.Structure):
+    """msc_ffn: the weights of a gated feed-forward block."""
+    _fields_ = [("dtype", C.c_int), ("hidden", C.c_int), ("act", C.c_int)] + [
+        (k, C.c_void_p) for k in ("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")]
+
+
+class FfnGrads(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("dx", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")]
+
+
+class FfnBlock(C.Structure):
+    """msc_ffn_block: x <- res_scale * x + gate * post(ffn(pre(x)))."""
+    _fields_ = [("ffn", Ffn), ("pre", Norm), ("post", Norm), ("gate", C.c_void_p), ("res_scale", C.c_float)]
 
 
 class SlabDesc(C.Structure):

@@ -18,6 +18,16 @@ refiner's operators with the reference's names and argument meaning
     quantize_topology_z(factor_coord, r)  -> zbin [h*w]           (:363-406)
     make_dense_image_level(zbin, w, h)    -> coords, nbr          (:274-310)
 
+Beside them, without a counterpart in the reference, the residual block that
+mixes each row's channels (a gated feed-forward block with the norms, gate
+and residual scale around it) and its backward pass:
+
+    gated_ffn(x, ffn, act)                -> y [n, c]
+    gated_ffn_backward(x, dy, ffn, act)   -> gradients
+    residual_norm(x, f, post, gate, pre)  -> r, h
+    residual_norm_backward(r, f, dr, dh)  -> gradients
+    ffn_stack(x, blocks)                  -> x (in place)
+
 ``SparseRefiner`` is the refiner itself (SparseRefiner, src/sparse.hpp:41-66):
 built from a MOGG image, ``refine_once`` updates log z of a point map in
 place with every step on the GPU.
@@ -38,6 +48,8 @@ from . import lib as L
 
 _DT = {torch.float32: L.MSC_F32, torch.float16: L.MSC_F16, torch.bfloat16: L.MSC_BF16}
 _WT = {"f32": L.MSC_W_F32, "f16": L.MSC_W_F16, "q8_0": L.MSC_W_Q8_0}
+_NORM = {"layer": L.MSC_NORM_LAYER, "rms": L.MSC_NORM_RMS}
+_ACT = {"silu": L.MSC_ACT_SILU, "gelu": L.MSC_ACT_GELU, "gelu_erf": L.MSC_ACT_GELU_ERF}
 
 
 def _p(t):
@@ -403,6 +415,175 @@ class SparseCudaExecutor:
                                         _DT[skip.dtype] if skip is not None else 0, _p(y), _DT[out_dtype], _p(ws),
                                         wsb, _stream()))
         return y
+
+    # ------------------------------------------- gated feed-forward blocks
+    def _need(self, t, name, shape, dtypes=(torch.float32,)):
+        """A contiguous tensor of this shape and type on this executor's device."""
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != self.device:
+            raise L.MscError(L.MSC_E_INVALID, f"{name} must be a tensor on cuda:{self.device}")
+        if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or not t.is_contiguous():
+            raise L.MscError(L.MSC_E_INVALID, f"{name} must be contiguous {list(shape)} of {[str(d) for d in dtypes]}, "
+                                              f"not {list(t.shape)} of {t.dtype}")
+        return t
+
+    def _rows(self, t, name):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[1] == 0:
+            raise L.MscError(L.MSC_E_INVALID, f"{name} must be a [n, c] tensor")
+        return self._need(t, name, t.shape, tuple(_DT))
+
+    def _scratch(self, nbytes: int) -> torch.Tensor:
+        """A workspace of this call alone: from the allocator's pool of the
+        current stream (or of the graph being captured), so that calls on two
+        streams or in two graphs never share one."""
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
+
+    def _norm(self, nrm, name, c):
+        if nrm is None:
+            return L.Norm(L.MSC_NORM_NONE, None, None, 0.0)
+        if nrm.get("kind") not in _NORM:
+            raise L.MscError(L.MSC_E_INVALID, f"{name} norm kind must be one of {sorted(_NORM)}")
+        w, b = nrm.get("w"), nrm.get("b")
+        for t, k in ((w, "w"), (b, "b")):
+            if t is not None:
+                self._need(t, f"{name} norm {k}", (c,))
+        return L.Norm(_NORM[nrm["kind"]], _p(w), _p(b), nrm.get("eps", 1e-6))
+
+    def _ffn(self, ffn: dict, act: str, c: int, dtype):
+        if act not in _ACT:
+            raise L.MscError(L.MSC_E_INVALID, f"act must be one of {sorted(_ACT)}")
+        hidden = ffn["w_gate"].shape[0]
+        self._need(ffn["w_gate"], "w_gate", (hidden, c), (dtype,))
+        self._need(ffn["w_up"], "w_up", (hidden, c), (dtype,))
+        self._need(ffn["w_down"], "w_down", (c, hidden), (dtype,))
+        for k, m in (("b_gate", hidden), ("b_up", hidden), ("b_down", c)):
+            if ffn.get(k) is not None:
+                self._need(ffn[k], k, (m,))
+        return L.Ffn(_DT[dtype], hidden, _ACT[act], *(_p(ffn.get(k)) for k in (
+            "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")))
+
+    def _residual(self, n, c, x_dtype, f_dtype, post, gate, pre, res_scale, coords):
+        d = L.ResidualNormDesc(c, _DT[x_dtype], _DT[f_dtype], self._norm(post, "post", c), self._norm(pre, "pre", c),
+                               _p(gate), self._samples(gate, "gate", n, c, coords), res_scale)
+        return d
+
+    def _samples(self, gate, name, n, c, coords) -> int:
+        """0 for a gate per channel, else the samples of a [nsamples, c] gate."""
+        if gate is None:
+            return 0
+        if gate.dim() == 1:
+            self._need(gate, name, (c,))
+            return 0
+        self._need(gate, name, (gate.shape[0], c))
+        if coords is None:
+            raise L.MscError(L.MSC_E_INVALID, f"a {name} per sample needs the coordinates")
+        self._need(coords, "coords", (n, 4), (torch.int32,))
+        return gate.shape[0]
+
+    def gated_ffn(self, x, ffn: dict, act: str = "silu", out=None):
+        """y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down
+        (msc_gated_ffn).  x [n, c] fp16 / bf16; ffn: w_gate, w_up [hidden, c]
+        and w_down [c, hidden] of x's type, b_gate, b_up, b_down float32 or
+        absent; out may be x."""
+        n, c = self._rows(x, "x").shape
+        f = self._ffn(ffn, act, c, x.dtype)
+        y = torch.empty_like(x) if out is None else self._need(out, "out", x.shape, (x.dtype,))
+        ws = self._scratch(self.lib.msc_gated_ffn_workspace_bytes(n, c, f.hidden))
+        L.check(self.lib.msc_gated_ffn(self.ctx, C.byref(f), n, c, _p(x), _p(y), _p(ws), ws.numel(), _stream()))
+        return y
+
+    def gated_ffn_backward(self, x, dy, ffn: dict, act: str = "silu", weights: bool = True) -> dict:
+        """Gradients of gated_ffn (msc_gated_ffn_backward): "x", with
+        ``weights`` also "w_gate", "w_up", "w_down" and the biases that the
+        block has."""
+        n, c = self._rows(x, "x").shape
+        self._need(dy, "dy", x.shape, (x.dtype,))
+        f = self._ffn(ffn, act, c, x.dtype)
+        out = {"x": torch.empty_like(x)}
+        if weights:
+            for k in ("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down"):
+                if ffn.get(k) is not None:
+                    out[k] = torch.empty_like(ffn[k])
+        g = L.FfnGrads(*(_p(out.get(k)) for k in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")))
+        ws = self._scratch(self.lib.msc_gated_ffn_backward_workspace_bytes(n, c, f.hidden))
+        L.check(self.lib.msc_gated_ffn_backward(self.ctx, C.byref(f), n, c, _p(x), _p(dy), C.byref(g), _p(ws),
+                                                ws.numel(), _stream()))
+        return out
+
+    def residual_norm(self, x, f=None, post=None, gate=None, pre=None, res_scale: float = 1.0, coords=None,
+                      branch_dtype=None, in_place: bool = False):
+        """r = res_scale * x + gate * post(f) and h = pre(r) in one pass
+        (msc_residual_norm); returns (r, h).
+
+        post, pre: dict(kind="layer" | "rms", w, b, eps) or None (no norm; h is
+        then None).  gate: [c], or [nsamples, c] with coords [n, 4] (sample in
+        field 3), or None.  x fp32 or of f's type; without f, h is of
+        ``branch_dtype`` (default x's).  in_place: r is x."""
+        n, c = self._rows(x, "x").shape
+        f_dtype = f.dtype if f is not None else (branch_dtype or x.dtype)
+        if f is not None:
+            self._need(f, "f", x.shape, (f_dtype,))
+        d = self._residual(n, c, x.dtype, f_dtype, post, gate if f is not None else None, pre, res_scale, coords)
+        r = x if in_place else torch.empty_like(x)
+        h = None if pre is None else torch.empty((n, c), dtype=f_dtype, device=x.device)
+        L.check(self.lib.msc_residual_norm(self.ctx, C.byref(d), n, _p(x), _p(f), _p(coords), _p(r), _p(h), _stream()))
+        return r, h
+
+    def residual_norm_backward(self, r, f, dr, dh, post=None, gate=None, pre=None, res_scale: float = 1.0,
+                               coords=None) -> dict:
+        """Gradients of residual_norm from its output r, the branch f and the
+        gradients dr and dh of its outputs (msc_residual_norm_backward): "x",
+        "f" and, where present, "gate", "post_w", "post_b", "pre_w", "pre_b".
+        dr may be None (zero); dh is None without a pre norm; f may be None."""
+        n, c = self._rows(r, "r").shape
+        f_dtype = f.dtype if f is not None else (dh.dtype if dh is not None else r.dtype)
+        if f is not None:
+            self._need(f, "f", r.shape, (f_dtype,))
+        if dr is not None:
+            self._need(dr, "dr", r.shape, (r.dtype,))
+        if dh is not None:
+            self._need(dh, "dh", r.shape, (f_dtype,))
+        if f is None:
+            post = gate = None
+        d = self._residual(n, c, r.dtype, f_dtype, post, gate, pre, res_scale, coords)
+        out = {"x": torch.empty_like(r)}
+        if f is not None:
+            out["f"] = torch.empty_like(f)
+        if gate is not None:
+            out["gate"] = torch.empty_like(gate)
+        for name, nrm in (("post", post), ("pre", pre)):
+            for k in ("w", "b"):
+                if nrm is not None and nrm.get(k) is not None:
+                    out[f"{name}_{k}"] = torch.empty_like(nrm[k])
+        g = L.ResidualNormGrads(*(_p(out.get(k)) for k in ("x", "f", "gate", "post_w", "post_b", "pre_w", "pre_b")))
+        ws = self._scratch(self.lib.msc_residual_norm_backward_workspace_bytes(n, c, d.nsamples))
+        L.check(self.lib.msc_residual_norm_backward(self.ctx, C.byref(d), n, _p(r), _p(f), _p(coords), _p(dr), _p(dh),
+                                                    C.byref(g), _p(ws), ws.numel(), _stream()))
+        return out
+
+    def ffn_stack(self, x, blocks: list, coords=None):
+        """In place on x [n, c]: x <- res_scale * x + gate * post(ffn(pre(x)))
+        per block (msc_ffn_stack).  A block: dict(ffn, act, pre, post, gate,
+        res_scale) with the parts of gated_ffn and residual_norm; x is fp32 or
+        of the weights' type."""
+        n, c = self._rows(x, "x").shape
+        arr = (L.FfnBlock * max(len(blocks), 1))()
+        nsamples, hidden = 0, 8
+        for i, b in enumerate(blocks):
+            dtype = b["ffn"]["w_gate"].dtype
+            ffn = self._ffn(b["ffn"], b.get("act", "silu"), c, dtype)
+            gate = b.get("gate")
+            ns = self._samples(gate, "gate", n, c, coords)
+            if gate is not None:
+                if i and nsamples != ns and any(p.get("gate") is not None for p in blocks[:i]):
+                    raise L.MscError(L.MSC_E_INVALID, "the gates of a stack are all per channel or of the same samples")
+                nsamples = ns
+            arr[i] = L.FfnBlock(ffn, self._norm(b.get("pre"), "pre", c), self._norm(b.get("post"), "post", c), _p(gate),
+                                b.get("res_scale", 1.0))
+            hidden = max(hidden, ffn.hidden)
+        ws = self._scratch(self.lib.msc_ffn_stack_workspace_bytes(n, c, hidden))
+        L.check(self.lib.msc_ffn_stack(self.ctx, _p(x), _DT[x.dtype], n, c, _p(coords), nsamples, len(blocks), arr,
+                                       _p(ws), ws.numel(), _stream()))
+        return x
 
 
 class SparseRefiner:
