@@ -60,41 +60,48 @@ __device__ __forceinline__ void zero8(Raw8<DT>& r) {
     for (int i = 0; i < (DT == DT_F32 ? 2 : 1); ++i) r.q[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// The 8 values as four f32 pairs (packed f32x2 arithmetic from here on: the
+// forward pass spends its instruction slots, not its memory time, on scalar
+// arithmetic otherwise).
 template <int DT>
-__device__ __forceinline__ void unpack8(const Raw8<DT>& r, float* v) {
+__device__ __forceinline__ void unpack8(const Raw8<DT>& r, uint64_t* v) {
     if constexpr (DT == DT_F32) {
-        const uint32_t w[8] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w, r.q[1].x, r.q[1].y, r.q[1].z, r.q[1].w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[e]);
+        v[0] = pack2(__uint_as_float(r.q[0].x), __uint_as_float(r.q[0].y));
+        v[1] = pack2(__uint_as_float(r.q[0].z), __uint_as_float(r.q[0].w));
+        v[2] = pack2(__uint_as_float(r.q[1].x), __uint_as_float(r.q[1].y));
+        v[3] = pack2(__uint_as_float(r.q[1].z), __uint_as_float(r.q[1].w));
     } else {
         const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float2 t;
-            if constexpr (DT == DT_F16)
-                t = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-            else
-                t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-            v[2 * e] = t.x, v[2 * e + 1] = t.y;
+            if constexpr (DT == DT_F16) {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                v[e] = pack2(t.x, t.y);
+            } else {
+                v[e] = pack2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+            }
         }
     }
 }
 
 template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t off, const float* v) {
+__device__ __forceinline__ void store8(void* p, int64_t off, const uint64_t* v) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) unpack2(v[e], f[2 * e], f[2 * e + 1]);
     if constexpr (DT == DT_F32) {
         float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + off);
-        d[0] = make_float4(v[0], v[1], v[2], v[3]);
-        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        d[0] = make_float4(f[0], f[1], f[2], f[3]);
+        d[1] = make_float4(f[4], f[5], f[6], f[7]);
     } else {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (DT == DT_F16) {
-                const __half2 h = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
                 w[e] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
                 w[e] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
@@ -102,37 +109,46 @@ __device__ __forceinline__ void store8(void* p, int64_t off, const float* v) {
     }
 }
 
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+__device__ __forceinline__ float sum_pair(uint64_t v) {
+    float a, b;
+    unpack2(v, a, b);
+    return a + b;
+}
+
 // 8 columns of a weight vector (fill where it is absent).
-__device__ __forceinline__ void load_param(const float* p, int col, float fill, float* v) {
+__device__ __forceinline__ void load_param(const float* p, int col, float fill, uint64_t* v) {
     if (p) {
         const float4 a = __ldg(reinterpret_cast<const float4*>(p + col));
         const float4 b = __ldg(reinterpret_cast<const float4*>(p + col) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        v[0] = pack2(a.x, a.y), v[1] = pack2(a.z, a.w), v[2] = pack2(b.x, b.y), v[3] = pack2(b.z, b.w);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fill;
+        for (int e = 0; e < 4; ++e) v[e] = both(fill);
     }
 }
 
-// Sums of a and b over the T threads of a row.  Beyond a warp the partial
+// Sums of a (and b) over the T threads of a row.  Beyond a warp the partial
 // sums cross through shared memory; `turn` alternates between two buffers, so
 // that one barrier per exchange orders both its own reads and the reuse.
-template <int T>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*buf)[T > 32 ? T / 32 : 1], int& turn) {
+template <int T, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float2 (*buf)[T > 32 ? T / 32 : 1], int& turn) {
 #pragma unroll
     for (int o = (T < 32 ? T : 32) / 2; o >= 1; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
     if constexpr (T > 32) {
-        if ((threadIdx.x & 31) == 0) buf[turn][threadIdx.x >> 5] = make_float2(a, b);
+        if ((threadIdx.x & 31) == 0) buf[turn][threadIdx.x >> 5] = make_float2(v[0], v[N - 1]);
         __syncthreads();
-        a = 0.f, b = 0.f;
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < T / 32; ++w) {
-            a += buf[turn][w].x;
-            b += buf[turn][w].y;
+            s.x += buf[turn][w].x;
+            s.y += buf[turn][w].y;
         }
+        v[0] = s.x;
+        if constexpr (N > 1) v[1] = s.y;
         turn ^= 1;
     }
 }
@@ -142,18 +158,19 @@ constexpr int block_threads() {
     return T > 32 ? T : 256;
 }
 
-// The row's gate: per channel, or of the row's sample.  An index outside the
-// samples is a device failure and gates the branch off.
-__device__ __forceinline__ int row_sample(const RowNormArgs& a, int64_t row, bool live) {
+// The sample of a row whose gate is per sample (0 otherwise, -1 where the
+// index is outside the samples: a device failure that gates the branch off).
+__device__ __forceinline__ int row_sample(const RowNormArgs& a, int64_t row) {
     if (!a.nsamples) return 0;
-    const int s = live ? __ldg(a.coords + row * 4 + 3) : 0;
-    if (static_cast<unsigned>(s) < static_cast<unsigned>(a.nsamples)) return s;
-    set_status(a.status, MSC_DEV_BAD_COORD);
-    return -1;
+    const int s = __ldg(a.coords + row * 4 + 3);
+    return static_cast<unsigned>(s) < static_cast<unsigned>(a.nsamples) ? s : -1;
 }
 
-template <int XT, int FT, int T, int V>
-__global__ void __launch_bounds__(block_threads<T>()) rownorm_kernel(const RowNormArgs a) {
+// Forward.  The gate folds into the post norm's weights (gate * (f^ w + b) =
+// f^ (gate w) + gate b), which are multiplied only when the gate changes; the
+// next step's row is on its way while this one is computed.
+template <int XT, int FT, int T, int V, bool FULL>
+__global__ void __launch_bounds__(block_threads<T>(), T > 32 ? (V > 1 ? 1 : 768 / T) : 3) rownorm_kernel(const RowNormArgs a) {
     constexpr int R = T > 32 ? 1 : 32 / T;  // rows per unit and step
     __shared__ float2 buf[2][T > 32 ? T / 32 : 1];
     int turn = 0;
@@ -162,115 +179,155 @@ __global__ void __launch_bounds__(block_threads<T>()) rownorm_kernel(const RowNo
     const int64_t unit = T > 32 ? blockIdx.x : blockIdx.x * (block_threads<T>() / 32) + (threadIdx.x >> 5);
     const int64_t units = T > 32 ? gridDim.x : static_cast<int64_t>(gridDim.x) * (block_threads<T>() / 32);
     const int chunks = a.c / 8;
+    // FULL: every thread has all its columns (c = 8 T V)
+    auto has = [&](int v) { return FULL || t + v * T < chunks; };
+    auto column = [&](int v) { return (FULL ? t + v * T : min(t + v * T, chunks - 1)) * 8; };
     const float inv_c = 1.0f / static_cast<float>(a.c);
-    float post_w[8], post_b[8], pre_w[8], pre_b[8], gate[8];
-    int gate_of = -2;  // sample whose gate is held
-    auto params = [&](int v) {
-        const int col = min(t + v * T, chunks - 1) * 8;
-        load_param(a.post.w, col, 1.f, post_w);
-        load_param(a.post.b, col, 0.f, post_b);
-        load_param(a.pre.w, col, 1.f, pre_w);
-        load_param(a.pre.b, col, 0.f, pre_b);
+    const bool has_post = a.post.kind != NORM_NONE;
+    uint64_t gate_w[V * 4], gate_b[V * 4];
+    int gate_of = -2;  // sample whose gate is folded in
+    const uint64_t scale = both(a.res_scale);
+    auto load_gate = [&](int s) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int col = column(v);
+            load_param(a.post.w, col, 1.f, gate_w + 4 * v);
+            load_param(a.post.b, col, 0.f, gate_b + 4 * v);
+            if (a.gate) {
+                uint64_t g[4];
+                load_param(s < 0 ? nullptr : a.gate + static_cast<int64_t>(s) * a.c, col, 0.f, g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    gate_w[4 * v + e] = mul2(gate_w[4 * v + e], g[e]);
+                    gate_b[4 * v + e] = mul2(gate_b[4 * v + e], g[e]);
+                }
+            }
+        }
+        gate_of = s;
     };
-    if constexpr (V == 1) params(0);
+    uint64_t pre_w[V * 4], pre_b[V * 4];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int col = column(v);
+        load_param(a.pre.w, col, 1.f, pre_w + 4 * v);
+        load_param(a.pre.b, col, 0.f, pre_b + 4 * v);
+    }
+    Raw8<XT> xr[V];
+    Raw8<FT> fr[V];
+    int s_next = 0;
+    // loads run without predicates: rows past the last one read the last one
+    // again, threads without a column the last columns, and both are left out
+    // of sums and stores
+    auto fetch = [&](int64_t row) {
+        row = min(row, a.n - 1);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t off = row * a.c + column(v);
+            xr[v] = load8<XT>(a.x, off);
+            if (a.f) fr[v] = load8<FT>(a.f, off);
+        }
+        s_next = row_sample(a, row);
+    };
+#pragma unroll
+    for (int v = 0; v < V; ++v) zero8(fr[v]);
+    fetch(unit * R + sub);
     for (int64_t row0 = unit * R; row0 < a.n; row0 += units * R) {
         const int64_t row = row0 + sub;
         const bool live = row < a.n;
-        Raw8<XT> xr[V];
-        Raw8<FT> fr[V];
+        uint64_t f[V * 4], r[V * 4];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            zero8(xr[v]);
-            zero8(fr[v]);
-            const int j = t + v * T;
-            if (live && j < chunks) {
-                xr[v] = load8<XT>(a.x, row * a.c + j * 8);
-                if (a.f) fr[v] = load8<FT>(a.f, row * a.c + j * 8);
-            }
+            unpack8(fr[v], f + 4 * v);
+            unpack8(xr[v], r + 4 * v);
         }
-        const int s = a.gate ? row_sample(a, row, live) : 0;
-        float r[V * 8];
-        float mean = 0.f, k = 1.f;
-        if (a.f && a.post.kind != NORM_NONE) {
-            float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                unpack8(fr[v], r + 8 * v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s1 += r[8 * v + e], s2 += r[8 * v + e] * r[8 * v + e];
-            }
-            if (a.post.kind == NORM_LAYER) {
+        const int s = s_next;
+        fetch(row + units * R);
+        if (s != gate_of) load_gate(s);
+        if (s < 0) set_status(a.status, MSC_DEV_BAD_COORD);
+        if (a.f) {
+            if (has_post) {
                 // two passes over the registers: the variance of the centred values
-                float dummy = 0.f;
-                row_sum2<T>(s1, dummy, buf, turn);
-                mean = s1 * inv_c;
-                s2 = 0.f;
+                float q[1] = {0.f};
+                if (a.post.kind == NORM_LAYER) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        uint64_t acc = 0ull;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc = add2(acc, f[4 * v + e]);
+                        if (has(v)) q[0] += sum_pair(acc);
+                    }
+                    row_sum<T>(q, buf, turn);
+                    const uint64_t m = both(-q[0] * inv_c);
+#pragma unroll
+                    for (int i = 0; i < V * 4; ++i) f[i] = add2(f[i], m);
+                }
+                q[0] = 0.f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    uint64_t acc = 0ull;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc = fma2(f[4 * v + e], f[4 * v + e], acc);
+                    if (has(v)) q[0] += sum_pair(acc);
+                }
+                row_sum<T>(q, buf, turn);
+                const uint64_t k = both(rsqrtf(q[0] * inv_c + a.post.eps));
+#pragma unroll
+                for (int i = 0; i < V * 4; ++i) f[i] = mul2(f[i], k);
+            }
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) r[i] = fma2(scale, r[i], fma2(f[i], gate_w[i], gate_b[i]));
+            if (s < 0) {
+                // the branch of a row without a sample stays out, whatever it holds
 #pragma unroll
                 for (int v = 0; v < V; ++v)
-                    if (t + v * T < chunks) {
+                    if (live && has(v)) {
+                        unpack8(load8<XT>(a.x, row * a.c + (t + v * T) * 8), r + 4 * v);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) s2 += (r[8 * v + e] - mean) * (r[8 * v + e] - mean);
+                        for (int e = 0; e < 4; ++e) r[4 * v + e] = mul2(scale, r[4 * v + e]);
                     }
             }
-            row_sum2<T>(s1, s2, buf, turn);
-            k = rsqrtf(s2 * inv_c + a.post.eps);
-        }
-        float s1 = 0.f, s2 = 0.f;
+        } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = t + v * T;
-            if constexpr (V > 1) params(v);
-            if (a.gate && (V > 1 || s != gate_of)) {
-                load_param(s < 0 ? nullptr : a.gate + static_cast<int64_t>(s) * a.c, min(j, chunks - 1) * 8, 0.f, gate);
-                gate_of = s;
-            }
-            float x[8], f[8];
-            unpack8(xr[v], x);
-            unpack8(fr[v], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float q = f[e];
-                if (a.post.kind != NORM_NONE) q = fmaf((q - mean) * k, post_w[e], post_b[e]);
-                if (a.gate) q *= gate[e];
-                q = a.f ? fmaf(a.res_scale, x[e], q) : a.res_scale * x[e];
-                r[8 * v + e] = j < chunks ? q : 0.f;
-                s1 += r[8 * v + e];
-                s2 += r[8 * v + e] * r[8 * v + e];
-            }
-            if (a.r && live && j < chunks) store8<XT>(a.r, row * a.c + j * 8, r + 8 * v);
+            for (int i = 0; i < V * 4; ++i) r[i] = mul2(scale, r[i]);
         }
-        if (a.pre.kind == NORM_NONE) {
-            // no norm: h, where asked for, is r in the branch's type
-            if (a.h && live) {
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (t + v * T < chunks) store8<FT>(a.h, row * a.c + (t + v * T) * 8, r + 8 * v);
-            }
-            continue;
-        }
-        mean = 0.f;
-        if (a.pre.kind == NORM_LAYER) {
-            float dummy = 0.f;
-            row_sum2<T>(s1, dummy, buf, turn);
-            mean = s1 * inv_c;
-            s2 = 0.f;
+        if (a.r && live) {
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                if (t + v * T < chunks) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s2 += (r[8 * v + e] - mean) * (r[8 * v + e] - mean);
-                }
+                if (has(v)) store8<XT>(a.r, row * a.c + (t + v * T) * 8, r + 4 * v);
         }
-        row_sum2<T>(s1, s2, buf, turn);
-        k = rsqrtf(s2 * inv_c + a.pre.eps);
+        if (a.pre.kind != NORM_NONE) {
+            float q[1] = {0.f};
+            if (a.pre.kind == NORM_LAYER) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = t + v * T;
-            if constexpr (V > 1) params(v);
-            float h[8];
+                for (int v = 0; v < V; ++v) {
+                    uint64_t acc = 0ull;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = fmaf((r[8 * v + e] - mean) * k, pre_w[e], pre_b[e]);
-            if (live && j < chunks) store8<FT>(a.h, row * a.c + j * 8, h);
+                    for (int e = 0; e < 4; ++e) acc = add2(acc, r[4 * v + e]);
+                    if (has(v)) q[0] += sum_pair(acc);
+                }
+                row_sum<T>(q, buf, turn);
+                const uint64_t m = both(-q[0] * inv_c);
+#pragma unroll
+                for (int i = 0; i < V * 4; ++i) r[i] = add2(r[i], m);
+            }
+            q[0] = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                uint64_t acc = 0ull;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = fma2(r[4 * v + e], r[4 * v + e], acc);
+                if (has(v)) q[0] += sum_pair(acc);
+            }
+            row_sum<T>(q, buf, turn);
+            const uint64_t k = both(rsqrtf(q[0] * inv_c + a.pre.eps));
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) r[i] = fma2(mul2(r[i], k), pre_w[i], pre_b[i]);
+        }
+        // without a norm h, where asked for, is r in the branch's type
+        if (a.h && live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (has(v)) store8<FT>(a.h, row * a.c + (t + v * T) * 8, r + 4 * v);
         }
     }
 }
@@ -278,7 +335,11 @@ __global__ void __launch_bounds__(block_threads<T>()) rownorm_kernel(const RowNo
 // Slab rows of a unit: pre_w, pre_b, post_w, post_b, then the gate's.
 enum SlabRow : int { SLAB_PRE_W = 0, SLAB_PRE_B = 1, SLAB_POST_W = 2, SLAB_POST_B = 3, SLAB_GATE = 4 };
 
-template <int XT, int FT, int T, int V>
+// Backward.  With one gate over a run of rows, the sums A = sum dr f^ and B =
+// sum dr give all three gradients of the branch (gate w A + b B, post norm's
+// weight gate A, its bias gate B), so only A and B are kept per row; they are
+// resolved into the unit's slab when the gate changes.
+template <int XT, int FT, int T, int V, bool FULL>
 __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rownorm_backward_kernel(const RowNormArgs a) {
     constexpr int R = T > 32 ? 1 : 32 / T;
     __shared__ float2 buf[2][T > 32 ? T / 32 : 1];
@@ -288,224 +349,293 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rown
     const int64_t unit = T > 32 ? blockIdx.x : blockIdx.x * (block_threads<T>() / 32) + (threadIdx.x >> 5);
     if (unit >= a.units) return;  // whole warps (T <= 32, no block barrier) or whole blocks
     const int chunks = a.c / 8;
+    // FULL: every thread has all its columns (c = 8 T V)
+    auto has = [&](int v) { return FULL || t + v * T < chunks; };
+    auto column = [&](int v) { return (FULL ? t + v * T : min(t + v * T, chunks - 1)) * 8; };
     const float inv_c = 1.0f / static_cast<float>(a.c);
-    const int gate_rows = !a.gate ? 0 : (a.nsamples ? a.nsamples : 1);
-    float* slab = a.partial + unit * (SLAB_GATE + gate_rows) * a.c;
+    const int slab_rows = SLAB_GATE + (!a.gate ? 0 : (a.nsamples ? a.nsamples : 1));
+    float* slab = a.partial + unit * slab_rows * a.c;
     const bool has_pre = a.pre.kind != NORM_NONE, has_post = a.post.kind != NORM_NONE;
-    float pre_w[8], post_w[8], post_b[8], gate[8];
-    int gate_of = -2;
-    auto params = [&](int v) {
-        const int col = min(t + v * T, chunks - 1) * 8;
-        load_param(a.pre.w, col, 1.f, pre_w);
-        load_param(a.post.w, col, 1.f, post_w);
-        load_param(a.post.b, col, 0.f, post_b);
+    const bool pre_ln = a.pre.kind == NORM_LAYER, post_ln = a.post.kind == NORM_LAYER;
+    const uint64_t scale = both(a.res_scale);
+    auto clear8 = [&](int srow, int col) {
+        float4* p = reinterpret_cast<float4*>(slab + static_cast<int64_t>(srow) * a.c + col);
+        p[0] = p[1] = make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    auto load_gate = [&](int v, int s) {
-        if (a.gate && (V > 1 || s != gate_of)) {
-            load_param(s < 0 ? nullptr : a.gate + static_cast<int64_t>(s) * a.c, min(t + v * T, chunks - 1) * 8, 0.f, gate);
-            gate_of = s;
-        }
-    };
-    if constexpr (V == 1) params(0);
-    float acc_pre_w[V * 8] = {}, acc_pre_b[V * 8] = {}, acc_post_w[V * 8] = {}, acc_post_b[V * 8] = {},
-          acc_gate[V * 8] = {};
-    int cur = -1;  // sample of the rows in acc_gate
-    // adds the rows held in acc_gate to the slab of their sample and clears them
-    auto flush_gate = [&]() {
+    if (sub == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
+            if (has(v))
+                for (int q = SLAB_POST_W; q < slab_rows; ++q) clear8(q, (t + v * T) * 8);
+    }
+    if constexpr (T <= 32) __syncwarp();
+    uint64_t pre_w[V * 4], gate_w[V * 4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float q = acc_gate[8 * v + e];
-                acc_gate[8 * v + e] = 0.f;
-                if constexpr (T < 32) {
+    for (int v = 0; v < V; ++v) load_param(a.pre.w, column(v), 1.f, pre_w + 4 * v);
+    auto load_gate8 = [&](int v, int s, uint64_t* g) {
+        if (a.gate)
+            load_param(s < 0 ? nullptr : a.gate + static_cast<int64_t>(s) * a.c, column(v), 0.f, g);
+        else
+            load_param(nullptr, 0, 1.f, g);
+    };
+    int gate_of = -2;
+    auto fold_gate = [&](int s) {
 #pragma unroll
-                    for (int o = T; o < 32; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-                }
-                if (cur >= 0 && sub == 0 && t + v * T < chunks) {
-                    float* p = slab + static_cast<int64_t>(SLAB_GATE + cur) * a.c + (t + v * T) * 8 + e;
-                    *p += q;
-                }
+        for (int v = 0; v < V; ++v) {
+            uint64_t g[4];
+            load_gate8(v, s, g);
+            load_param(a.post.w, column(v), 1.f, gate_w + 4 * v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gate_w[4 * v + e] = mul2(gate_w[4 * v + e], g[e]);
+        }
+        gate_of = s;
+    };
+    uint64_t acc_pre_w[V * 4], acc_pre_b[V * 4], acc_a[V * 4], acc_b[V * 4];
+#pragma unroll
+    for (int i = 0; i < V * 4; ++i) acc_pre_w[i] = acc_pre_b[i] = acc_a[i] = acc_b[i] = 0ull;
+    auto add8 = [&](int srow, int col, const uint64_t* v) {
+        float* p = slab + static_cast<int64_t>(srow) * a.c + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float lo, hi;
+            unpack2(v[e], lo, hi);
+            p[2 * e] += lo;
+            p[2 * e + 1] += hi;
+        }
+    };
+    // adds A and B of rows of sample s to the slab (by the calling lanes)
+    auto resolve = [&](int v, int s, const uint64_t* sa, const uint64_t* sb) {
+        const int col = (t + v * T) * 8;
+        if (!has(v) || s < 0) return;
+        uint64_t g[4], w[4], o[4];
+        load_gate8(v, s, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = mul2(g[e], sa[e]);
+        add8(SLAB_POST_W, col, o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = mul2(g[e], sb[e]);
+        add8(SLAB_POST_B, col, o);
+        if (!a.gate) return;
+        load_param(a.post.b, col, 0.f, g);
+        load_param(a.post.w, col, 1.f, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fma2(w[e], sa[e], mul2(g[e], sb[e]));
+        add8(SLAB_GATE + s, col, o);
+    };
+    auto over_rows = [&](uint64_t* v) {  // sum over the warp's rows
+        if constexpr (T < 32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int o = T; o < 32; o <<= 1) v[e] = add2(v[e], __shfl_xor_sync(0xffffffffu, v[e], o));
             }
+        }
+    };
+    int cur = -1;  // sample of the rows in A and B
+    auto flush = [&]() {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            over_rows(acc_a + 4 * v);
+            over_rows(acc_b + 4 * v);
+            if (sub == 0) resolve(v, cur, acc_a + 4 * v, acc_b + 4 * v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc_a[4 * v + e] = acc_b[4 * v + e] = 0ull;
+        }
         if constexpr (T <= 32) __syncwarp();
     };
     const int64_t row_end = min(a.n, (unit + 1) * a.rows_per_unit);
+    Raw8<XT> rr[V], gr[V];
+    Raw8<FT> fr[V], hr[V];
+    int s_next = 0;
+    auto fetch = [&](int64_t row) {
+        row = min(row, row_end - 1);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t off = row * a.c + column(v);
+            if (has_pre) rr[v] = load8<XT>(a.x, off);
+            if (a.dh) hr[v] = load8<FT>(a.dh, off);
+            if (a.dr) gr[v] = load8<XT>(a.dr, off);
+            if (a.f) fr[v] = load8<FT>(a.f, off);
+        }
+        s_next = row_sample(a, row);
+    };
+#pragma unroll
+    for (int v = 0; v < V; ++v) zero8(rr[v]), zero8(gr[v]), zero8(fr[v]), zero8(hr[v]);
+    fetch(unit * a.rows_per_unit + sub);
     for (int64_t row0 = unit * a.rows_per_unit; row0 < row_end; row0 += R) {
         const int64_t row = row0 + sub;
         const bool live = row < row_end;
-        Raw8<XT> rr[V], gr[V];
-        Raw8<FT> fr[V], hr[V];
+        uint64_t r[V * 4], f[V * 4], d[V * 4], g[V * 4];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            zero8(rr[v]), zero8(gr[v]), zero8(fr[v]), zero8(hr[v]);
-            const int j = t + v * T;
-            if (live && j < chunks) {
-                const int64_t off = row * a.c + j * 8;
-                if (has_pre) rr[v] = load8<XT>(a.x, off);
-                if (a.dh) hr[v] = load8<FT>(a.dh, off);
-                if (a.dr) gr[v] = load8<XT>(a.dr, off);
-                if (a.f) fr[v] = load8<FT>(a.f, off);
+            unpack8(rr[v], r + 4 * v);
+            unpack8(fr[v], f + 4 * v);
+            unpack8(hr[v], d + 4 * v);
+            unpack8(gr[v], g + 4 * v);
+        }
+        const int s = s_next;
+        fetch(row + R);
+        if (!live) {
+            // past the run: nothing to add
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) d[i] = g[i] = 0ull;
+        }
+        if (s != gate_of) fold_gate(s);
+        if (s < 0) {
+            // a row without a sample has no branch
+            set_status(a.status, MSC_DEV_BAD_COORD);
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) f[i] = 0ull;
+        }
+        // the rows' gate changes: resolve the sums so far
+        bool mixed = false;
+        {
+            int first = s;
+            if constexpr (T < 32) {
+                first = __shfl_sync(0xffffffffu, s, 0);  // the first row of a step is always live
+                mixed = !__all_sync(0xffffffffu, s == first);
+            }
+            if (mixed || first != cur) {
+                flush();
+                cur = mixed ? -1 : first;
             }
         }
-        const int s = a.gate ? row_sample(a, row, live) : 0;
         // both norms' statistics together: means, then centred squares
-        float r_mean = 0.f, f_mean = 0.f, s1 = 0.f, s2 = 0.f;
-        float r[V * 8], f[V * 8];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            unpack8(rr[v], r + 8 * v);
-            unpack8(fr[v], f + 8 * v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s1 += r[8 * v + e], s2 += f[8 * v + e];
-        }
-        if (a.pre.kind == NORM_LAYER || a.post.kind == NORM_LAYER) {
-            row_sum2<T>(s1, s2, buf, turn);
-            if (a.pre.kind == NORM_LAYER) r_mean = s1 * inv_c;
-            if (a.post.kind == NORM_LAYER) f_mean = s2 * inv_c;
-        }
-        s1 = s2 = 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (t + v * T < chunks) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    r[8 * v + e] -= r_mean;
-                    if (has_post) f[8 * v + e] -= f_mean;
-                    s1 += r[8 * v + e] * r[8 * v + e];
-                    s2 += f[8 * v + e] * f[8 * v + e];
-                }
-            }
-        row_sum2<T>(s1, s2, buf, turn);
-        const float r_k = rsqrtf(s1 * inv_c + a.pre.eps);
-        const float f_k = has_post ? rsqrtf(s2 * inv_c + a.post.eps) : 1.f;
-        // dr = dr + norm'_pre(dh; r)
-        float d[V * 8];
-        s1 = s2 = 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if constexpr (V > 1) params(v);
-            float g[8];
-            unpack8(hr[v], g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = 8 * v + e;
-                r[i] *= r_k;
-                if (has_pre) {
-                    acc_pre_w[i] = fmaf(g[e], r[i], acc_pre_w[i]);
-                    acc_pre_b[i] += g[e];
-                }
-                d[i] = has_pre ? g[e] * pre_w[e] : g[e];
-                s1 += d[i];
-                s2 = fmaf(d[i], r[i], s2);
-            }
-        }
-        if (has_pre) row_sum2<T>(s1, s2, buf, turn);
-        const float m1 = a.pre.kind == NORM_LAYER ? s1 * inv_c : 0.f, m2 = s2 * inv_c;
-        float q1 = 0.f, q2 = 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int j = t + v * T;
-            if constexpr (V > 1) params(v);
-            load_gate(v, s);
-            float g[8], o[8];
-            unpack8(gr[v], g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = 8 * v + e;
-                g[e] = has_pre ? fmaf(r_k, d[i] - m1 - r[i] * m2, g[e]) : g[e] + d[i];
-                o[e] = a.res_scale * g[e];
-                f[i] *= f_k;  // f^, or f without a norm
-                const float tt = has_post ? fmaf(f[i], post_w[e], post_b[e]) : f[i];
-                r[i] = g[e] * tt;  // this row's gate gradient
-                const float dt = a.gate ? gate[e] * g[e] : g[e];
-                acc_post_w[i] = fmaf(dt, f[i], acc_post_w[i]);
-                acc_post_b[i] += dt;
-                d[i] = has_post ? dt * post_w[e] : dt;
-                q1 += d[i];
-                q2 = fmaf(d[i], f[i], q2);
-            }
-            if (a.dx && live && j < chunks) store8<XT>(a.dx, row * a.c + j * 8, o);
-        }
-        if (a.f) {
-            if (has_post) row_sum2<T>(q1, q2, buf, turn);
-            const float n1 = a.post.kind == NORM_LAYER ? q1 * inv_c : 0.f, n2 = q2 * inv_c;
+        float q[2] = {0.f, 0.f};
+        if (pre_ln || post_ln) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int j = t + v * T;
+                uint64_t u0 = 0ull, u1 = 0ull;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u0 = add2(u0, r[4 * v + e]), u1 = add2(u1, f[4 * v + e]);
+                if (has(v)) q[0] += sum_pair(u0), q[1] += sum_pair(u1);
+            }
+            row_sum<T>(q, buf, turn);
+            const uint64_t rm = both(pre_ln ? -q[0] * inv_c : 0.f), fm = both(post_ln ? -q[1] * inv_c : 0.f);
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) r[i] = add2(r[i], rm), f[i] = add2(f[i], fm);
+            q[0] = q[1] = 0.f;
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            uint64_t u0 = 0ull, u1 = 0ull;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                u0 = fma2(r[4 * v + e], r[4 * v + e], u0), u1 = fma2(f[4 * v + e], f[4 * v + e], u1);
+            if (has(v)) q[0] += sum_pair(u0), q[1] += sum_pair(u1);
+        }
+        row_sum<T>(q, buf, turn);
+        const float r_k = rsqrtf(q[0] * inv_c + a.pre.eps);
+        const float f_k = has_post ? rsqrtf(q[1] * inv_c + a.post.eps) : 1.f;
+        // dr = dr + norm'_pre(dh; r)
+        if (has_pre) {
+            const uint64_t k2 = both(r_k);
+            q[0] = q[1] = 0.f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                uint64_t u0 = 0ull, u1 = 0ull;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * v + e;
+                    r[i] = mul2(r[i], k2);
+                    acc_pre_w[i] = fma2(d[i], r[i], acc_pre_w[i]);
+                    acc_pre_b[i] = add2(acc_pre_b[i], d[i]);
+                    d[i] = mul2(d[i], pre_w[i]);
+                    u0 = add2(u0, d[i]);
+                    u1 = fma2(d[i], r[i], u1);
+                }
+                if (has(v)) q[0] += sum_pair(u0), q[1] += sum_pair(u1);
+            }
+            row_sum<T>(q, buf, turn);
+            const uint64_t m1 = both(pre_ln ? -q[0] * inv_c : 0.f), m2 = both(-q[1] * inv_c);
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) g[i] = fma2(k2, add2(fma2(r[i], m2, d[i]), m1), g[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) g[i] = add2(g[i], d[i]);
+        }
+        if (a.dx && live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (has(v)) {
+                    uint64_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = mul2(scale, g[4 * v + e]);
+                    store8<XT>(a.dx, row * a.c + (t + v * T) * 8, o);
+                }
+        }
+        if (!a.f) continue;
+        const uint64_t k2 = both(f_k);
+        q[0] = q[1] = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            uint64_t u0 = 0ull, u1 = 0ull;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * v + e;
+                f[i] = mul2(f[i], k2);  // f^, or f without a norm
+                d[i] = mul2(g[i], gate_w[i]);
+                u0 = add2(u0, d[i]);
+                u1 = fma2(d[i], f[i], u1);
+            }
+            if (has(v)) q[0] += sum_pair(u0), q[1] += sum_pair(u1);
+        }
+        if (mixed) {
+            // the step's rows belong to different samples: one row after the other
+            for (int k = 0; k < R; ++k) {
+                if (sub == k && live) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        uint64_t u0[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u0[e] = mul2(g[4 * v + e], f[4 * v + e]);
+                        resolve(v, s, u0, g + 4 * v);
+                    }
+                }
+                __syncwarp();
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) acc_a[i] = fma2(g[i], f[i], acc_a[i]), acc_b[i] = add2(acc_b[i], g[i]);
+        }
+        if (has_post) {
+            row_sum<T>(q, buf, turn);
+            const uint64_t n1 = both(post_ln ? -q[0] * inv_c : 0.f), n2 = both(-q[1] * inv_c);
+#pragma unroll
+            for (int i = 0; i < V * 4; ++i) d[i] = mul2(k2, add2(fma2(f[i], n2, d[i]), n1));
+        }
+        if (a.df && live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (has(v)) store8<FT>(a.df, row * a.c + (t + v * T) * 8, d + 4 * v);
+        }
+    }
+    flush();
+    auto put = [&](uint64_t* acc, int srow) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            over_rows(acc + 4 * v);
+            if (sub == 0 && has(v)) {
                 float o[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int i = 8 * v + e;
-                    o[e] = has_post ? f_k * (d[i] - n1 - f[i] * n2) : d[i];
-                }
-                if (a.df && live && j < chunks) store8<FT>(a.df, row * a.c + j * 8, o);
+                for (int e = 0; e < 4; ++e) unpack2(acc[4 * v + e], o[2 * e], o[2 * e + 1]);
+                float4* p = reinterpret_cast<float4*>(slab + static_cast<int64_t>(srow) * a.c + (t + v * T) * 8);
+                p[0] = make_float4(o[0], o[1], o[2], o[3]);
+                p[1] = make_float4(o[4], o[5], o[6], o[7]);
             }
         }
-        if (a.gate) {
-            if (a.nsamples) {
-                int first = s;
-                bool mixed = false;
-                if constexpr (T < 32) {
-                    first = __shfl_sync(0xffffffffu, s, 0);  // the first row of a step is always live
-                    mixed = !__all_sync(0xffffffffu, !live || s == first);
-                }
-                if (mixed || first != cur) {
-                    flush_gate();
-                    cur = mixed ? -1 : first;
-                }
-                if (mixed) {
-                    // the step's rows belong to different samples: one row after the other
-                    for (int g = 0; g < R; ++g) {
-                        if (sub == g && live && s >= 0) {
-#pragma unroll
-                            for (int v = 0; v < V; ++v)
-                                if (t + v * T < chunks) {
-                                    float* p = slab + static_cast<int64_t>(SLAB_GATE + s) * a.c + (t + v * T) * 8;
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) p[e] += r[8 * v + e];
-                                }
-                        }
-                        __syncwarp();
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V * 8; ++i) acc_gate[i] += live ? r[i] : 0.f;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V * 8; ++i) acc_gate[i] += r[i];
-            }
-        }
-    }
-    if (a.gate) {
-        if (!a.nsamples) cur = 0;
-        flush_gate();
-    }
-    auto put = [&](float* acc, int slab_row) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float q = acc[8 * v + e];
-                if constexpr (T < 32) {
-#pragma unroll
-                    for (int o = T; o < 32; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-                }
-                if (sub == 0 && t + v * T < chunks)
-                    slab[static_cast<int64_t>(slab_row) * a.c + (t + v * T) * 8 + e] = q;
-            }
     };
     put(acc_pre_w, SLAB_PRE_W);
     put(acc_pre_b, SLAB_PRE_B);
-    put(acc_post_w, SLAB_POST_W);
-    put(acc_post_b, SLAB_POST_B);
 }
 
-// Column sums over the units, 32 columns a block, in double and in a fixed order.
+// Column sums over the units, 8 columns (a 32-byte sector) a block, in double
+// and in a fixed order.
 __global__ void __launch_bounds__(1024) slab_sum_kernel(const float* part, int64_t units, int slab_rows, int c,
                                                         RowNormGrads g) {
-    __shared__ double red[32][33];
-    const int col = blockIdx.x * 32 + threadIdx.x;
+    __shared__ double red[128][9];
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int col = blockIdx.x * 8 + tx;
     const int srow = blockIdx.y;
     float* dst = nullptr;
     if (srow == SLAB_PRE_W) dst = g.pre_w;
@@ -515,15 +645,15 @@ __global__ void __launch_bounds__(1024) slab_sum_kernel(const float* part, int64
     else if (g.gate) dst = g.gate + static_cast<int64_t>(srow - SLAB_GATE) * c;
     if (!dst) return;
     double s = 0.0;
-    if (col < c)
-        for (int64_t u = threadIdx.y; u < units; u += 32) s += part[(u * slab_rows + srow) * c + col];
-    red[threadIdx.y][threadIdx.x] = s;
+#pragma unroll 8
+    for (int64_t u = ty; u < units; u += 128) s += part[(u * slab_rows + srow) * c + col];
+    red[ty][tx] = s;
     __syncthreads();
-    for (int o = 16; o >= 1; o >>= 1) {
-        if (threadIdx.y < o) red[threadIdx.y][threadIdx.x] += red[threadIdx.y + o][threadIdx.x];
+    for (int o = 64; o >= 1; o >>= 1) {
+        if (ty < o) red[ty][tx] += red[ty + o][tx];
         __syncthreads();
     }
-    if (threadIdx.y == 0 && col < c) dst[col] = static_cast<float>(red[0][threadIdx.x]);
+    if (ty == 0) dst[col] = static_cast<float>(red[0][tx]);
 }
 
 int sm_count() {
@@ -564,28 +694,31 @@ void backward_units(int64_t n, int c, int nsamples, int64_t* units, int64_t* row
     *units = std::max<int64_t>((n + *rows_per_unit - 1) / *rows_per_unit, 1);
 }
 
-template <int XT, int FT, int T, int V>
+template <int XT, int FT, int T, int V, bool FULL>
 cudaError_t launch_fwd(const RowNormArgs& a, cudaStream_t st) {
     constexpr int threads = block_threads<T>();
     constexpr int rows = T > 32 ? 1 : threads / T;  // rows a block and step
     const int64_t blocks = (a.n + rows - 1) / rows;
-    const int64_t cap = static_cast<int64_t>(sm_count()) * (2048 / threads);
-    rownorm_kernel<XT, FT, T, V><<<static_cast<unsigned>(std::min(blocks, cap)), threads, 0, st>>>(a);
+    const int64_t cap = static_cast<int64_t>(sm_count()) * std::max(768 / threads, 1);
+    rownorm_kernel<XT, FT, T, V, FULL><<<static_cast<unsigned>(std::min(blocks, cap)), threads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
-template <int XT, int FT, int T, int V>
+template <int XT, int FT, int T, int V, bool FULL>
 cudaError_t launch_bwd(const RowNormArgs& a, cudaStream_t st) {
     constexpr int threads = block_threads<T>();
     constexpr int per_block = T > 32 ? 1 : threads / 32;
-    rownorm_backward_kernel<XT, FT, T, V>
+    rownorm_backward_kernel<XT, FT, T, V, FULL>
         <<<static_cast<unsigned>((a.units + per_block - 1) / per_block), threads, 0, st>>>(a);
     return cudaGetLastError();
 }
 
 template <int XT, int FT>
 cudaError_t launch_c(const RowNormArgs& a, bool backward, cudaStream_t st) {
-#define MSC_ROWNORM_CASE(T, V) return backward ? launch_bwd<XT, FT, T, V>(a, st) : launch_fwd<XT, FT, T, V>(a, st)
+#define MSC_ROWNORM_CASE(T, V)                                                                               \
+    if (a.c == 8 * T * V)                                                                                    \
+        return backward ? launch_bwd<XT, FT, T, V, true>(a, st) : launch_fwd<XT, FT, T, V, true>(a, st);     \
+    return backward ? launch_bwd<XT, FT, T, V, false>(a, st) : launch_fwd<XT, FT, T, V, false>(a, st)
     switch (row_threads(a.c)) {
         case 8: MSC_ROWNORM_CASE(8, 1);
         case 16: MSC_ROWNORM_CASE(16, 1);
@@ -594,7 +727,9 @@ cudaError_t launch_c(const RowNormArgs& a, bool backward, cudaStream_t st) {
         case 128: MSC_ROWNORM_CASE(128, 1);
         default: break;
     }
-    if (a.c <= 2048) MSC_ROWNORM_CASE(256, 1);
+    if (a.c <= 2048) {
+        MSC_ROWNORM_CASE(256, 1);
+    }
     MSC_ROWNORM_CASE(512, 2);
 #undef MSC_ROWNORM_CASE
 }
@@ -627,8 +762,7 @@ cudaError_t launch_rownorm_backward(RowNormArgs a, const RowNormGrads& g, void* 
     a.partial = static_cast<float*>(ws);
     backward_units(a.n, a.c, a.nsamples, &a.units, &a.rows_per_unit);
     const int slab_rows = SLAB_GATE + (!a.gate ? 0 : (a.nsamples ? a.nsamples : 1));
-    // the gate rows are added to, so they start at zero (all rows do where n = 0)
-    if (a.gate || a.n == 0) {
+    if (a.n == 0) {
         cudaError_t e = cudaMemsetAsync(ws, 0, static_cast<size_t>(a.units) * slab_rows * a.c * sizeof(float), st);
         if (e != cudaSuccess) return e;
     }
@@ -636,7 +770,7 @@ cudaError_t launch_rownorm_backward(RowNormArgs a, const RowNormGrads& g, void* 
         cudaError_t e = launch_any(a, true, st);
         if (e != cudaSuccess) return e;
     }
-    slab_sum_kernel<<<dim3((a.c + 31) / 32, slab_rows), dim3(32, 32), 0, st>>>(a.partial, a.units, slab_rows, a.c, g);
+    slab_sum_kernel<<<dim3(a.c / 8, slab_rows), 1024, 0, st>>>(a.partial, a.units, slab_rows, a.c, g);
     return cudaGetLastError();
 }
 
