@@ -35,6 +35,7 @@
 #include "conv.h"
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 namespace msc {
@@ -55,10 +56,63 @@ __device__ __forceinline__ Raw8<DT> load8(const void* p, int64_t off) {
 }
 
 template <int DT>
-__device__ __forceinline__ void zero8(Raw8<DT>& r) {
+__device__ __forceinline__ Raw8<DT> zero8() {
+    Raw8<DT> r;
 #pragma unroll
     for (int i = 0; i < (DT == DT_F32 ? 2 : 1); ++i) r.q[i] = make_uint4(0u, 0u, 0u, 0u);
+    return r;
 }
+
+// Rows on their way from global memory: a ring of up to four steps in shared
+// memory, filled by 16-byte cp.async.  Every thread copies and reads its own
+// pieces alone, so that no barrier is needed, only its own wait.  BYTES is a
+// thread's share of the SM's shared memory at the kernel's occupancy.
+
+template <int DT>
+constexpr int pieces() {
+    return DT == DT_F32 ? 2 : 1;
+}
+
+// [step][piece][thread] 16-byte pieces, then [step][thread] sample indices.
+template <int THREADS, int PIECES, int BYTES>
+struct Ring {
+    uint32_t base;  // shared-window address of this thread's first piece
+    static constexpr int FIT = BYTES / (PIECES * 16 + 4);
+    static constexpr int DEPTH = FIT > 4 ? 4 : FIT;
+    static_assert(DEPTH >= 1, "one step fits");
+    static constexpr size_t bytes() { return static_cast<size_t>(DEPTH) * THREADS * (PIECES * 16 + 4); }
+    __device__ __forceinline__ explicit Ring(void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
+    __device__ __forceinline__ uint32_t at(int slot, int piece) const {
+        return base + static_cast<uint32_t>((slot * PIECES + piece) * THREADS * 16);
+    }
+    __device__ __forceinline__ uint32_t sample_at(int slot) const {
+        return base - threadIdx.x * 12 + static_cast<uint32_t>(DEPTH * PIECES * THREADS * 16 + slot * THREADS * 4);
+    }
+    template <int DT>
+    __device__ __forceinline__ void put(int slot, int piece, const void* p, int64_t off) const {
+        const uint8_t* src = static_cast<const uint8_t*>(p) + off * (DT == DT_F32 ? 4 : 2);
+#pragma unroll
+        for (int i = 0; i < pieces<DT>(); ++i) cp_async16(at(slot, piece + i), src + 16 * i, 16);
+    }
+    template <int DT>
+    __device__ __forceinline__ Raw8<DT> get(int slot, int piece) const {
+        Raw8<DT> r;
+#pragma unroll
+        for (int i = 0; i < pieces<DT>(); ++i)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(r.q[i].x), "=r"(r.q[i].y), "=r"(r.q[i].z), "=r"(r.q[i].w)
+                         : "r"(at(slot, piece + i)));
+        return r;
+    }
+    __device__ __forceinline__ void put_sample(int slot, const int32_t* p) const {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sample_at(slot)), "l"(p) : "memory");
+    }
+    __device__ __forceinline__ int get_sample(int slot) const {
+        int s;
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(s) : "r"(sample_at(slot)));
+        return s;
+    }
+};
 
 // The 8 values as four f32 pairs (packed f32x2 arithmetic from here on: the
 // forward pass spends its instruction slots, not its memory time, on scalar
@@ -158,13 +212,16 @@ constexpr int block_threads() {
     return T > 32 ? T : 256;
 }
 
-// The sample of a row whose gate is per sample (0 otherwise, -1 where the
-// index is outside the samples: a device failure that gates the branch off).
-__device__ __forceinline__ int row_sample(const RowNormArgs& a, int64_t row) {
-    if (!a.nsamples) return 0;
-    const int s = __ldg(a.coords + row * 4 + 3);
+// 0 where the gate is not per sample, -1 where the index is outside the
+// samples: a device failure that gates the branch off.
+__device__ __forceinline__ int checked_sample(const RowNormArgs& a, int s) {
     return static_cast<unsigned>(s) < static_cast<unsigned>(a.nsamples) ? s : -1;
 }
+
+template <int XT, int FT, int T, int V>
+using FwdRing = Ring<block_threads<T>(), V * (pieces<XT>() + pieces<FT>()), 290>;
+template <int XT, int FT, int T, int V>
+using BwdRing = Ring<block_threads<T>(), 2 * V * (pieces<XT>() + pieces<FT>()), 430>;
 
 // Forward.  The gate folds into the post norm's weights (gate * (f^ w + b) =
 // f^ (gate w) + gate b), which are multiplied only when the gate changes; the
@@ -212,36 +269,39 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? (V > 1 ? 1 : 768 
         load_param(a.pre.w, col, 1.f, pre_w + 4 * v);
         load_param(a.pre.b, col, 0.f, pre_b + 4 * v);
     }
-    Raw8<XT> xr[V];
-    Raw8<FT> fr[V];
-    int s_next = 0;
     // loads run without predicates: rows past the last one read the last one
     // again, threads without a column the last columns, and both are left out
     // of sums and stores
-    auto fetch = [&](int64_t row) {
+    extern __shared__ uint4 ring_smem[];
+    const FwdRing<XT, FT, T, V> ring(ring_smem);
+    constexpr int D = FwdRing<XT, FT, T, V>::DEPTH;
+    constexpr int PX = pieces<XT>(), PF = pieces<FT>();
+    auto fetch = [&](int slot, int64_t row) {
         row = min(row, a.n - 1);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int64_t off = row * a.c + column(v);
-            xr[v] = load8<XT>(a.x, off);
-            if (a.f) fr[v] = load8<FT>(a.f, off);
+            ring.template put<XT>(slot, v * PX, a.x, off);
+            if (a.f) ring.template put<FT>(slot, V * PX + v * PF, a.f, off);
         }
-        s_next = row_sample(a, row);
+        if (a.nsamples) ring.put_sample(slot, a.coords + row * 4 + 3);
+        cp_async_commit();
     };
 #pragma unroll
-    for (int v = 0; v < V; ++v) zero8(fr[v]);
-    fetch(unit * R + sub);
-    for (int64_t row0 = unit * R; row0 < a.n; row0 += units * R) {
+    for (int k = 0; k < D - 1; ++k) fetch(k, (unit + k * units) * R + sub);
+    int slot = 0;
+    for (int64_t row0 = unit * R; row0 < a.n; row0 += units * R, slot = (slot + 1) % D) {
         const int64_t row = row0 + sub;
         const bool live = row < a.n;
+        fetch((slot + D - 1) % D, row + (D - 1) * units * R);
+        cp_async_wait<D - 1>();
         uint64_t f[V * 4], r[V * 4];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            unpack8(fr[v], f + 4 * v);
-            unpack8(xr[v], r + 4 * v);
+            unpack8(ring.template get<XT>(slot, v * PX), r + 4 * v);
+            unpack8(a.f ? ring.template get<FT>(slot, V * PX + v * PF) : zero8<FT>(), f + 4 * v);
         }
-        const int s = s_next;
-        fetch(row + units * R);
+        const int s = a.nsamples ? checked_sample(a, ring.get_sample(slot)) : 0;
         if (s != gate_of) load_gate(s);
         if (s < 0) set_status(a.status, MSC_DEV_BAD_COORD);
         if (a.f) {
@@ -444,37 +504,41 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rown
         if constexpr (T <= 32) __syncwarp();
     };
     const int64_t row_end = min(a.n, (unit + 1) * a.rows_per_unit);
-    Raw8<XT> rr[V], gr[V];
-    Raw8<FT> fr[V], hr[V];
-    int s_next = 0;
-    auto fetch = [&](int64_t row) {
+    extern __shared__ uint4 ring_smem[];
+    const BwdRing<XT, FT, T, V> ring(ring_smem);
+    constexpr int D = BwdRing<XT, FT, T, V>::DEPTH;
+    constexpr int PX = pieces<XT>(), PF = pieces<FT>();
+    constexpr int P_GR = V * PX, P_FR = 2 * V * PX, P_HR = P_FR + V * PF;
+    auto fetch = [&](int slot, int64_t row) {
         row = min(row, row_end - 1);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int64_t off = row * a.c + column(v);
-            if (has_pre) rr[v] = load8<XT>(a.x, off);
-            if (a.dh) hr[v] = load8<FT>(a.dh, off);
-            if (a.dr) gr[v] = load8<XT>(a.dr, off);
-            if (a.f) fr[v] = load8<FT>(a.f, off);
+            if (has_pre) ring.template put<XT>(slot, v * PX, a.x, off);
+            if (a.dr) ring.template put<XT>(slot, P_GR + v * PX, a.dr, off);
+            if (a.f) ring.template put<FT>(slot, P_FR + v * PF, a.f, off);
+            if (a.dh) ring.template put<FT>(slot, P_HR + v * PF, a.dh, off);
         }
-        s_next = row_sample(a, row);
+        if (a.nsamples) ring.put_sample(slot, a.coords + row * 4 + 3);
+        cp_async_commit();
     };
 #pragma unroll
-    for (int v = 0; v < V; ++v) zero8(rr[v]), zero8(gr[v]), zero8(fr[v]), zero8(hr[v]);
-    fetch(unit * a.rows_per_unit + sub);
-    for (int64_t row0 = unit * a.rows_per_unit; row0 < row_end; row0 += R) {
+    for (int k = 0; k < D - 1; ++k) fetch(k, unit * a.rows_per_unit + k * R + sub);
+    int slot = 0;
+    for (int64_t row0 = unit * a.rows_per_unit; row0 < row_end; row0 += R, slot = (slot + 1) % D) {
         const int64_t row = row0 + sub;
         const bool live = row < row_end;
+        fetch((slot + D - 1) % D, row + (D - 1) * R);
+        cp_async_wait<D - 1>();
         uint64_t r[V * 4], f[V * 4], d[V * 4], g[V * 4];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            unpack8(rr[v], r + 4 * v);
-            unpack8(fr[v], f + 4 * v);
-            unpack8(hr[v], d + 4 * v);
-            unpack8(gr[v], g + 4 * v);
+            unpack8(has_pre ? ring.template get<XT>(slot, v * PX) : zero8<XT>(), r + 4 * v);
+            unpack8(a.dr ? ring.template get<XT>(slot, P_GR + v * PX) : zero8<XT>(), g + 4 * v);
+            unpack8(a.f ? ring.template get<FT>(slot, P_FR + v * PF) : zero8<FT>(), f + 4 * v);
+            unpack8(a.dh ? ring.template get<FT>(slot, P_HR + v * PF) : zero8<FT>(), d + 4 * v);
         }
-        const int s = s_next;
-        fetch(row + R);
+        const int s = a.nsamples ? checked_sample(a, ring.get_sample(slot)) : 0;
         if (!live) {
             // past the run: nothing to add
 #pragma unroll
@@ -694,22 +758,42 @@ void backward_units(int64_t n, int c, int nsamples, int64_t* units, int64_t* row
     *units = std::max<int64_t>((n + *rows_per_unit - 1) / *rows_per_unit, 1);
 }
 
+// Shared-memory opt-in of a kernel, once per device.
+cudaError_t smem_opt_in(const void* kern, size_t smem, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done.load(std::memory_order_acquire) >> dev & 1) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e == cudaSuccess) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    return e;
+}
+
 template <int XT, int FT, int T, int V, bool FULL>
 cudaError_t launch_fwd(const RowNormArgs& a, cudaStream_t st) {
     constexpr int threads = block_threads<T>();
+    constexpr size_t smem = FwdRing<XT, FT, T, V>::bytes();
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(rownorm_kernel<XT, FT, T, V, FULL>), smem, done);
+    if (e != cudaSuccess) return e;
     constexpr int rows = T > 32 ? 1 : threads / T;  // rows a block and step
     const int64_t blocks = (a.n + rows - 1) / rows;
     const int64_t cap = static_cast<int64_t>(sm_count()) * std::max(768 / threads, 1);
-    rownorm_kernel<XT, FT, T, V, FULL><<<static_cast<unsigned>(std::min(blocks, cap)), threads, 0, st>>>(a);
+    rownorm_kernel<XT, FT, T, V, FULL><<<static_cast<unsigned>(std::min(blocks, cap)), threads, smem, st>>>(a);
     return cudaGetLastError();
 }
 
 template <int XT, int FT, int T, int V, bool FULL>
 cudaError_t launch_bwd(const RowNormArgs& a, cudaStream_t st) {
     constexpr int threads = block_threads<T>();
+    constexpr size_t smem = BwdRing<XT, FT, T, V>::bytes();
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = smem_opt_in(reinterpret_cast<const void*>(rownorm_backward_kernel<XT, FT, T, V, FULL>), smem, done);
+    if (e != cudaSuccess) return e;
     constexpr int per_block = T > 32 ? 1 : threads / 32;
     rownorm_backward_kernel<XT, FT, T, V, FULL>
-        <<<static_cast<unsigned>((a.units + per_block - 1) / per_block), threads, 0, st>>>(a);
+        <<<static_cast<unsigned>((a.units + per_block - 1) / per_block), threads, smem, st>>>(a);
     return cudaGetLastError();
 }
 
