@@ -367,6 +367,13 @@ __device__ __forceinline__ uint64_t silu2(uint64_t v2) {
     return mul2(v2, pack2(r0, r1));
 }
 
+// Programmatic dependent launch: lets the next kernel of the stream start
+// its prologue; waits until the kernels before have finished and their
+// writes are visible (returns at once in a kernel launched without the
+// attribute).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 
 }  // namespace msc

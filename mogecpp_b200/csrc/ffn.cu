@@ -15,6 +15,7 @@
 
 #include "conv.h"
 #include "ffn_gemm.cuh"
+#include "ffn_rows.h"
 
 #include <algorithm>
 #include <cstring>
@@ -261,6 +262,10 @@ struct FwdWs {
 };
 FwdWs fwd_ws(int64_t n, int c, int hidden) {
     FwdWs w{};
+    if (n <= kFfnFewRows) {
+        w.total = align256(static_cast<size_t>(n) * hidden * 4);
+        return w;
+    }
     const ProjPlan p = proj_plan(n, c, static_cast<int>(cdiv(hidden, 64)));
     w.hidden = 0;
     w.part = align256(static_cast<size_t>(n) * hidden * 2);
@@ -310,6 +315,7 @@ size_t ffn_backward_workspace_bytes(int64_t n, int c, int hidden) { return bwd_w
 cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, void* y, void* ws, uint32_t* status,
                        cudaStream_t st) {
     if (s.n == 0) return cudaSuccess;
+    if (s.n <= kFfnFewRows) return launch_ffn_rows(s, x, w, y, static_cast<float*>(ws), st);
     const bool bf = s.dtype == DT_BF16;
     const FwdWs o = fwd_ws(s.n, s.c, s.hidden);
     char* base = static_cast<char*>(ws);

@@ -49,11 +49,19 @@ from . import lib as L
 _DT = {torch.float32: L.MSC_F32, torch.float16: L.MSC_F16, torch.bfloat16: L.MSC_BF16}
 _WT = {"f32": L.MSC_W_F32, "f16": L.MSC_W_F16, "q8_0": L.MSC_W_Q8_0}
 _NORM = {"layer": L.MSC_NORM_LAYER, "rms": L.MSC_NORM_RMS}
+_F32_ONLY = (torch.float32,)
+_NO_NORM = L.Norm(L.MSC_NORM_NONE, None, None, 0.0)
+_FFN_KEYS = ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")
+_RES_KEYS = ("x", "f", "gate", "post_w", "post_b", "pre_w", "pre_b")
 _ACT = {"silu": L.MSC_ACT_SILU, "gelu": L.MSC_ACT_GELU, "gelu_erf": L.MSC_ACT_GELU_ERF}
 
 
 def _p(t):
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _stream():
@@ -417,54 +425,62 @@ class SparseCudaExecutor:
         return y
 
     # ------------------------------------------- gated feed-forward blocks
-    def _need(self, t, name, shape, dtypes=(torch.float32,)):
+    # The wrappers below pass addresses as plain integers and the stream
+    # handle straight from torch's C layer: on rows this few the host side of
+    # a call costs more than its kernels.
+    def _need(self, t, name, shape, dtypes=_F32_ONLY):
         """A contiguous tensor of this shape and type on this executor's device."""
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != self.device:
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.device:
             raise L.MscError(L.MSC_E_INVALID, f"{name} must be a tensor on cuda:{self.device}")
-        if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or not t.is_contiguous():
+        if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous():
             raise L.MscError(L.MSC_E_INVALID, f"{name} must be contiguous {list(shape)} of {[str(d) for d in dtypes]}, "
                                               f"not {list(t.shape)} of {t.dtype}")
-        return t
+        return t.data_ptr()
+
+    def _need_opt(self, t, name, shape, dtypes=_F32_ONLY):
+        return None if t is None else self._need(t, name, shape, dtypes)
 
     def _rows(self, t, name):
         if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[1] == 0:
             raise L.MscError(L.MSC_E_INVALID, f"{name} must be a [n, c] tensor")
-        return self._need(t, name, t.shape, tuple(_DT))
+        self._need(t, name, t.shape, _DT)
+        return t.shape
 
-    def _scratch(self, nbytes: int) -> torch.Tensor:
+    def _raw_stream(self) -> int:
+        return torch._C._cuda_getCurrentRawStream(self.device)
+
+    @staticmethod
+    def _scratch(like, nbytes: int) -> torch.Tensor:
         """A workspace of this call alone: from the allocator's pool of the
         current stream (or of the graph being captured), so that calls on two
         streams or in two graphs never share one."""
-        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=f"cuda:{self.device}")
+        return like.new_empty(max(nbytes, 256), dtype=torch.uint8)
 
     def _norm(self, nrm, name, c):
         if nrm is None:
-            return L.Norm(L.MSC_NORM_NONE, None, None, 0.0)
-        if nrm.get("kind") not in _NORM:
+            return _NO_NORM
+        kind = _NORM.get(nrm.get("kind"))
+        if kind is None:
             raise L.MscError(L.MSC_E_INVALID, f"{name} norm kind must be one of {sorted(_NORM)}")
-        w, b = nrm.get("w"), nrm.get("b")
-        for t, k in ((w, "w"), (b, "b")):
-            if t is not None:
-                self._need(t, f"{name} norm {k}", (c,))
-        return L.Norm(_NORM[nrm["kind"]], _p(w), _p(b), nrm.get("eps", 1e-6))
+        shape = (c,)
+        return L.Norm(kind, self._need_opt(nrm.get("w"), f"{name} norm w", shape),
+                      self._need_opt(nrm.get("b"), f"{name} norm b", shape), nrm.get("eps", 1e-6))
 
     def _ffn(self, ffn: dict, act: str, c: int, dtype):
         if act not in _ACT:
             raise L.MscError(L.MSC_E_INVALID, f"act must be one of {sorted(_ACT)}")
-        hidden = ffn["w_gate"].shape[0]
-        self._need(ffn["w_gate"], "w_gate", (hidden, c), (dtype,))
-        self._need(ffn["w_up"], "w_up", (hidden, c), (dtype,))
-        self._need(ffn["w_down"], "w_down", (c, hidden), (dtype,))
-        for k, m in (("b_gate", hidden), ("b_up", hidden), ("b_down", c)):
-            if ffn.get(k) is not None:
-                self._need(ffn[k], k, (m,))
-        return L.Ffn(_DT[dtype], hidden, _ACT[act], *(_p(ffn.get(k)) for k in (
-            "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")))
+        hidden, dt = ffn["w_gate"].shape[0], (dtype,)
+        return L.Ffn(_DT[dtype], hidden, _ACT[act], self._need(ffn["w_gate"], "w_gate", (hidden, c), dt),
+                     self._need(ffn["w_up"], "w_up", (hidden, c), dt),
+                     self._need(ffn["w_down"], "w_down", (c, hidden), dt),
+                     self._need_opt(ffn.get("b_gate"), "b_gate", (hidden,)),
+                     self._need_opt(ffn.get("b_up"), "b_up", (hidden,)),
+                     self._need_opt(ffn.get("b_down"), "b_down", (c,)))
 
     def _residual(self, n, c, x_dtype, f_dtype, post, gate, pre, res_scale, coords):
-        d = L.ResidualNormDesc(c, _DT[x_dtype], _DT[f_dtype], self._norm(post, "post", c), self._norm(pre, "pre", c),
-                               _p(gate), self._samples(gate, "gate", n, c, coords), res_scale)
-        return d
+        return L.ResidualNormDesc(c, _DT[x_dtype], _DT[f_dtype], self._norm(post, "post", c), self._norm(pre, "pre", c),
+                                  None if gate is None else gate.data_ptr(),
+                                  self._samples(gate, "gate", n, c, coords), res_scale)
 
     def _samples(self, gate, name, n, c, coords) -> int:
         """0 for a gate per channel, else the samples of a [nsamples, c] gate."""
@@ -484,29 +500,32 @@ class SparseCudaExecutor:
         (msc_gated_ffn).  x [n, c] fp16 / bf16; ffn: w_gate, w_up [hidden, c]
         and w_down [c, hidden] of x's type, b_gate, b_up, b_down float32 or
         absent; out may be x."""
-        n, c = self._rows(x, "x").shape
+        n, c = self._rows(x, "x")
         f = self._ffn(ffn, act, c, x.dtype)
-        y = torch.empty_like(x) if out is None else self._need(out, "out", x.shape, (x.dtype,))
-        ws = self._scratch(self.lib.msc_gated_ffn_workspace_bytes(n, c, f.hidden))
-        L.check(self.lib.msc_gated_ffn(self.ctx, C.byref(f), n, c, _p(x), _p(y), _p(ws), ws.numel(), _stream()))
-        return y
+        if out is None:
+            out = torch.empty_like(x)
+        y = self._need(out, "out", x.shape, (x.dtype,))
+        ws = self._scratch(x, self.lib.msc_gated_ffn_workspace_bytes(n, c, f.hidden))
+        L.check(self.lib.msc_gated_ffn(self.ctx, C.byref(f), n, c, x.data_ptr(), y, ws.data_ptr(), ws.numel(),
+                                       self._raw_stream()))
+        return out
 
     def gated_ffn_backward(self, x, dy, ffn: dict, act: str = "silu", weights: bool = True) -> dict:
         """Gradients of gated_ffn (msc_gated_ffn_backward): "x", with
         ``weights`` also "w_gate", "w_up", "w_down" and the biases that the
         block has."""
-        n, c = self._rows(x, "x").shape
+        n, c = self._rows(x, "x")
         self._need(dy, "dy", x.shape, (x.dtype,))
         f = self._ffn(ffn, act, c, x.dtype)
         out = {"x": torch.empty_like(x)}
         if weights:
-            for k in ("w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down"):
+            for k in _FFN_KEYS[1:]:
                 if ffn.get(k) is not None:
                     out[k] = torch.empty_like(ffn[k])
-        g = L.FfnGrads(*(_p(out.get(k)) for k in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")))
-        ws = self._scratch(self.lib.msc_gated_ffn_backward_workspace_bytes(n, c, f.hidden))
-        L.check(self.lib.msc_gated_ffn_backward(self.ctx, C.byref(f), n, c, _p(x), _p(dy), C.byref(g), _p(ws),
-                                                ws.numel(), _stream()))
+        g = L.FfnGrads(*[out[k].data_ptr() if k in out else None for k in _FFN_KEYS])
+        ws = self._scratch(x, self.lib.msc_gated_ffn_backward_workspace_bytes(n, c, f.hidden))
+        L.check(self.lib.msc_gated_ffn_backward(self.ctx, C.byref(f), n, c, x.data_ptr(), dy.data_ptr(), C.byref(g),
+                                                ws.data_ptr(), ws.numel(), self._raw_stream()))
         return out
 
     def residual_norm(self, x, f=None, post=None, gate=None, pre=None, res_scale: float = 1.0, coords=None,
@@ -518,14 +537,18 @@ class SparseCudaExecutor:
         then None).  gate: [c], or [nsamples, c] with coords [n, 4] (sample in
         field 3), or None.  x fp32 or of f's type; without f, h is of
         ``branch_dtype`` (default x's).  in_place: r is x."""
-        n, c = self._rows(x, "x").shape
-        f_dtype = f.dtype if f is not None else (branch_dtype or x.dtype)
-        if f is not None:
-            self._need(f, "f", x.shape, (f_dtype,))
-        d = self._residual(n, c, x.dtype, f_dtype, post, gate if f is not None else None, pre, res_scale, coords)
+        n, c = self._rows(x, "x")
+        if f is None:
+            f_dtype, gate = branch_dtype or x.dtype, None
+        else:
+            f_dtype = f.dtype
+            self._need(f, "f", x.shape, _DT)
+        d = self._residual(n, c, x.dtype, f_dtype, post, gate, pre, res_scale, coords)
         r = x if in_place else torch.empty_like(x)
-        h = None if pre is None else torch.empty((n, c), dtype=f_dtype, device=x.device)
-        L.check(self.lib.msc_residual_norm(self.ctx, C.byref(d), n, _p(x), _p(f), _p(coords), _p(r), _p(h), _stream()))
+        h = None if pre is None else (torch.empty_like(x) if f_dtype == x.dtype else x.new_empty((n, c), dtype=f_dtype))
+        L.check(self.lib.msc_residual_norm(self.ctx, C.byref(d), n, x.data_ptr(), _ptr(f),
+                                           coords.data_ptr() if d.nsamples else None, r.data_ptr(), _ptr(h),
+                                           self._raw_stream()))
         return r, h
 
     def residual_norm_backward(self, r, f, dr, dh, post=None, gate=None, pre=None, res_scale: float = 1.0,
@@ -534,16 +557,15 @@ class SparseCudaExecutor:
         gradients dr and dh of its outputs (msc_residual_norm_backward): "x",
         "f" and, where present, "gate", "post_w", "post_b", "pre_w", "pre_b".
         dr may be None (zero); dh is None without a pre norm; f may be None."""
-        n, c = self._rows(r, "r").shape
-        f_dtype = f.dtype if f is not None else (dh.dtype if dh is not None else r.dtype)
-        if f is not None:
-            self._need(f, "f", r.shape, (f_dtype,))
-        if dr is not None:
-            self._need(dr, "dr", r.shape, (r.dtype,))
-        if dh is not None:
-            self._need(dh, "dh", r.shape, (f_dtype,))
+        n, c = self._rows(r, "r")
         if f is None:
+            f_dtype = dh.dtype if dh is not None else r.dtype
             post = gate = None
+        else:
+            f_dtype = f.dtype
+            self._need(f, "f", r.shape, _DT)
+        self._need_opt(dr, "dr", r.shape, (r.dtype,))
+        self._need_opt(dh, "dh", r.shape, (f_dtype,))
         d = self._residual(n, c, r.dtype, f_dtype, post, gate, pre, res_scale, coords)
         out = {"x": torch.empty_like(r)}
         if f is not None:
@@ -551,13 +573,15 @@ class SparseCudaExecutor:
         if gate is not None:
             out["gate"] = torch.empty_like(gate)
         for name, nrm in (("post", post), ("pre", pre)):
-            for k in ("w", "b"):
-                if nrm is not None and nrm.get(k) is not None:
-                    out[f"{name}_{k}"] = torch.empty_like(nrm[k])
-        g = L.ResidualNormGrads(*(_p(out.get(k)) for k in ("x", "f", "gate", "post_w", "post_b", "pre_w", "pre_b")))
-        ws = self._scratch(self.lib.msc_residual_norm_backward_workspace_bytes(n, c, d.nsamples))
-        L.check(self.lib.msc_residual_norm_backward(self.ctx, C.byref(d), n, _p(r), _p(f), _p(coords), _p(dr), _p(dh),
-                                                    C.byref(g), _p(ws), ws.numel(), _stream()))
+            if nrm is not None:
+                for k in ("w", "b"):
+                    if nrm.get(k) is not None:
+                        out[f"{name}_{k}"] = torch.empty_like(nrm[k])
+        g = L.ResidualNormGrads(*[out[k].data_ptr() if k in out else None for k in _RES_KEYS])
+        ws = self._scratch(r, self.lib.msc_residual_norm_backward_workspace_bytes(n, c, d.nsamples))
+        L.check(self.lib.msc_residual_norm_backward(self.ctx, C.byref(d), n, r.data_ptr(), _ptr(f),
+                                                    coords.data_ptr() if d.nsamples else None, _ptr(dr), _ptr(dh),
+                                                    C.byref(g), ws.data_ptr(), ws.numel(), self._raw_stream()))
         return out
 
     def ffn_stack(self, x, blocks: list, coords=None):
@@ -565,11 +589,13 @@ class SparseCudaExecutor:
         per block (msc_ffn_stack).  A block: dict(ffn, act, pre, post, gate,
         res_scale) with the parts of gated_ffn and residual_norm; x is fp32 or
         of the weights' type."""
-        n, c = self._rows(x, "x").shape
+        n, c = self._rows(x, "x")
         arr = (L.FfnBlock * max(len(blocks), 1))()
         nsamples, hidden = 0, 8
         for i, b in enumerate(blocks):
             dtype = b["ffn"]["w_gate"].dtype
+            if dtype not in _DT:
+                raise L.MscError(L.MSC_E_INVALID, f"feed-forward weights of {dtype} are not supported")
             ffn = self._ffn(b["ffn"], b.get("act", "silu"), c, dtype)
             gate = b.get("gate")
             ns = self._samples(gate, "gate", n, c, coords)
@@ -577,12 +603,12 @@ class SparseCudaExecutor:
                 if i and nsamples != ns and any(p.get("gate") is not None for p in blocks[:i]):
                     raise L.MscError(L.MSC_E_INVALID, "the gates of a stack are all per channel or of the same samples")
                 nsamples = ns
-            arr[i] = L.FfnBlock(ffn, self._norm(b.get("pre"), "pre", c), self._norm(b.get("post"), "post", c), _p(gate),
+            arr[i] = L.FfnBlock(ffn, self._norm(b.get("pre"), "pre", c), self._norm(b.get("post"), "post", c), _ptr(gate),
                                 b.get("res_scale", 1.0))
             hidden = max(hidden, ffn.hidden)
-        ws = self._scratch(self.lib.msc_ffn_stack_workspace_bytes(n, c, hidden))
-        L.check(self.lib.msc_ffn_stack(self.ctx, _p(x), _DT[x.dtype], n, c, _p(coords), nsamples, len(blocks), arr,
-                                       _p(ws), ws.numel(), _stream()))
+        ws = self._scratch(x, self.lib.msc_ffn_stack_workspace_bytes(n, c, hidden))
+        L.check(self.lib.msc_ffn_stack(self.ctx, x.data_ptr(), _DT[x.dtype], n, c,
+                                       _ptr(coords) if nsamples else None, nsamples, len(blocks), arr, ws.data_ptr(), ws.numel(), self._raw_stream()))
         return x
 
 
