@@ -20,9 +20,9 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libmoge_sparse_cuda.so")
 SOURCES = ["topology.cu", "prep.cu", "gn.cu", "conv_tc.cu", "plan.cu", "ops.cu", "capi.cu",
            "noalloc.cu", "image_topo.cu", "refiner.cu", "slab.cu", "rownorm.cu", "ffn.cu",
-           "ffn_rows.cu"]
+           "ffn_rows.cu", "ffn_fused.cu"]
 HEADERS = ["common.cuh", "conv.h", "conv_common.cuh", "gn.h", "ops.h", "plan.h", "topology.h", "image_topo.h",
-           "rownorm.h", "ffn.h", "ffn_act.cuh", "ffn_rows.h", "ffn_gemm.cuh", "tma.cuh"]
+           "rownorm.h", "ffn.h", "ffn_act.cuh", "ffn_rows.h", "ffn_fused.h", "ffn_gemm.cuh", "tma.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
          "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr", "-I", os.path.join(ROOT, "include")]

@@ -14,6 +14,7 @@
 #include "ffn.h"
 
 #include "conv.h"
+#include "ffn_fused.h"
 #include "ffn_gemm.cuh"
 #include "ffn_rows.h"
 
@@ -257,11 +258,16 @@ cudaError_t launch_column_total(const float* part, int64_t units, int cols, int 
         if (e_ != cudaSuccess) return e_;    \
     } while (0)
 
+// One kernel for the whole block where the channels fit its accumulators and
+// the rows fill the SMs with 256-row tiles.
+bool use_fused(int64_t n, int c) { return c <= kFfnFusedMaxC && n >= kFfnFusedMinRows; }
+
 struct FwdWs {
     size_t hidden, part, total;
 };
 FwdWs fwd_ws(int64_t n, int c, int hidden) {
     FwdWs w{};
+    if (use_fused(n, c)) return w;
     if (n <= kFfnFewRows) {
         w.total = align256(static_cast<size_t>(n) * hidden * 4);
         return w;
@@ -315,6 +321,7 @@ size_t ffn_backward_workspace_bytes(int64_t n, int c, int hidden) { return bwd_w
 cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, void* y, void* ws, uint32_t* status,
                        cudaStream_t st) {
     if (s.n == 0) return cudaSuccess;
+    if (use_fused(s.n, s.c)) return launch_ffn_fused(s, x, w, y, status, st);
     if (s.n <= kFfnFewRows) return launch_ffn_rows(s, x, w, y, static_cast<float*>(ws), st);
     const bool bf = s.dtype == DT_BF16;
     const FwdWs o = fwd_ws(s.n, s.c, s.hidden);

@@ -1,0 +1,410 @@
+// Gated feed-forward block of many rows and few channels (c <= 128) in one
+// kernel: the hidden values never leave the SM.
+//
+// With c channels a hidden value costs 6 c flops but, written out and read
+// back, 4 bytes of HBM traffic: at c = 128 that traffic (and the store path)
+// takes longer than the products.  Here a CTA keeps two 128-row subtiles of x
+// in shared memory and walks the hidden units in chunks of 64:
+//   D = x [Wg chunk | Wu chunk]^T   (TMEM, 128 rows x 128 columns, K = c)
+//   h = act(D_g + bg) * (D_u + bu)  (epilogue warps -> shared memory, 16 bits)
+//   Y += h Wd[:, chunk]^T           (TMEM, 128 rows x c columns, K = 64)
+// The weights stream through shared memory once per 256 rows (they stay in
+// L2).  The two subtiles run half a chunk apart: while the epilogue warps of
+// one turn D into h, the tensor core works on the other, and each subtile's
+// next D is issued before its Y so that its epilogue can go on at once.
+//
+// TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 MMA
+// issuer, 2 TMEM allocation, 4-19 epilogue (8 per subtile: lane quarter x
+// half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
+#include "ffn_fused.h"
+
+#include "common.cuh"
+#include "conv.h"
+#include "conv_common.cuh"
+#include "ffn_act.cuh"
+#include "ffn_gemm.cuh"
+#include "tma.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+namespace msc {
+namespace {
+
+constexpr int kThreads = 640;
+constexpr int kGroupWarps = 8;  // epilogue warps of a subtile
+
+// KC: 64-channel blocks of a row (c padded with zeros by the copies).
+template <int KC>
+struct FusedCfg {
+    static constexpr int XR = KC == 1 ? 4 : 2;   // x subtile slots
+    static constexpr int W1R = KC == 1 ? 4 : 3;  // gate and up weight stages
+    static constexpr int W2R = KC == 1 ? 4 : 2;  // down weight stages
+    static constexpr int X_BYTES = KC * 128 * 128;
+    static constexpr int W1_BYTES = KC * 128 * 128;  // per 64-channel block: 64 gate rows, then 64 up rows
+    static constexpr int W2_BYTES = KC * 64 * 128;   // c rows of 64 hidden units
+    static constexpr int H_BYTES = 128 * 128;
+    static constexpr int CP = KC * 64;  // padded channels
+    static constexpr int SMEM = 1024 + XR * X_BYTES + W1R * W1_BYTES + W2R * W2_BYTES + 2 * H_BYTES + 512;
+    static_assert(SMEM <= kFfnSmemMax, "shared memory budget");
+};
+
+struct alignas(64) FusedArgs {
+    CUtensorMap mx, mg, mu, md, my;
+    int tiles, chunks;  // 256-row tiles, 64-unit hidden chunks
+    int rows, c, hidden;
+    const float* b_gate;
+    const float* b_up;
+    const float* b_down;
+    int act, bf16;
+    uint32_t* status;
+};
+
+struct FusedSmem {
+    uint8_t *x, *w1, *w2, *h;
+    uint64_t *x_full, *x_empty, *w1_full, *w1_empty, *w2_full, *w2_empty;
+    uint64_t *d_full, *h_ready, *h_free, *y_full, *y_empty, *drained;  // per subtile
+    uint32_t* tmem;
+    int* abort;
+};
+
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+
+template <int KC>
+__device__ void fused_producer(const FusedArgs& a, const FusedSmem& S) {
+    using C = FusedCfg<KC>;
+    int ix = 0, i1 = 0, i2 = 0;
+    // waits until `slot` of a ring is free for its i-th use
+    auto free_slot = [&](uint64_t* empty, int i, int ring) {
+        return i < ring ||
+               wait_or_abort(&empty[i % ring], static_cast<uint32_t>(i / ring - 1) & 1, S.abort, a.status);
+    };
+    auto load_w1 = [&](int j) {
+        if (!free_slot(S.w1_empty, i1, C::W1R)) return false;
+        const int s = i1++ % C::W1R;
+        const uint32_t dst = smem_u32(S.w1 + s * C::W1_BYTES);
+        mbar_arrive_expect_tx(&S.w1_full[s], C::W1_BYTES);
+#pragma unroll
+        for (int kb = 0; kb < KC; ++kb) {
+            tma_load_2d(dst + kb * 16384, &a.mg, kb * 64, j * 64, &S.w1_full[s]);
+            tma_load_2d(dst + kb * 16384 + 8192, &a.mu, kb * 64, j * 64, &S.w1_full[s]);
+        }
+        return true;
+    };
+    auto run = [&]() {
+        for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+            if (!load_w1(0)) return false;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub, ++ix) {
+                if (!free_slot(S.x_empty, ix, C::XR)) return false;
+                const int s = ix % C::XR;
+                mbar_arrive_expect_tx(&S.x_full[s], C::X_BYTES);
+#pragma unroll
+                for (int kb = 0; kb < KC; ++kb)
+                    tma_load_2d(smem_u32(S.x + s * C::X_BYTES + kb * 16384), &a.mx, kb * 64, tile * 256 + sub * 128,
+                                &S.x_full[s]);
+            }
+            // the next tile's rows on their way to L2
+            if (tile + static_cast<int>(gridDim.x) < a.tiles)
+#pragma unroll
+                for (int kb = 0; kb < 2 * KC; ++kb)
+                    tma_prefetch_2d(&a.mx, (kb % KC) * 64, (tile + static_cast<int>(gridDim.x)) * 256 + kb / KC * 128);
+            for (int j = 0; j < a.chunks; ++j) {
+                if (!free_slot(S.w2_empty, i2, C::W2R)) return false;
+                const int s = i2++ % C::W2R;
+                mbar_arrive_expect_tx(&S.w2_full[s], C::W2_BYTES);
+                tma_load_2d(smem_u32(S.w2 + s * C::W2_BYTES), &a.md, j * 64, 0, &S.w2_full[s]);
+                if (j + 1 < a.chunks && !load_w1(j + 1)) return false;
+            }
+        }
+        return true;
+    };
+    if (!run()) {
+        // aborted: copies in flight land within microseconds; wait 100 us
+        // before the CTA's shared memory can go away
+        const uint64_t t_end = global_timer_ns() + 100000ull;
+        while (global_timer_ns() < t_end) __nanosleep(1000);
+    }
+}
+
+template <int KC>
+__device__ void fused_issuer(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
+    using C = FusedCfg<KC>;
+    const uint32_t fmt = a.bf16 ? 1u : 0u;
+    const uint32_t idesc1 = idesc_f16(128, 128, fmt), idesc2 = idesc_f16(128, C::CP, fmt);
+    int ix = 0, i1 = 0, i2 = 0, c = 0, k = 0;  // x slots, weight stages, chunks and tiles so far
+    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k, ix += 2) {
+        auto product1 = [&](int sub, int stage) {
+            const uint32_t sx = smem_u32(S.x + ((ix + sub) % C::XR) * C::X_BYTES);
+            const uint32_t sw = smem_u32(S.w1 + stage * C::W1_BYTES);
+#pragma unroll
+            for (int ks = 0; ks < KC * 4; ++ks) {
+                const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
+                umma_f16(tmem + 256 + sub * 128, sdesc_k_sw128(sx + off), sdesc_k_sw128(sw + off), idesc1, ks > 0 ? 1u : 0u);
+            }
+            umma_commit(&S.d_full[sub]);
+        };
+        // first chunk of both subtiles
+        if (!wait(&S.w1_full[i1 % C::W1R], i1 / C::W1R)) return;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            if (!wait(&S.x_full[(ix + sub) % C::XR], (ix + sub) / C::XR)) return;
+            tc_fence_after();
+            product1(sub, i1 % C::W1R);
+            if (a.chunks == 1) umma_commit(&S.x_empty[(ix + sub) % C::XR]);
+        }
+        umma_commit(&S.w1_empty[i1 % C::W1R]);
+        ++i1;
+        for (int j = 0; j < a.chunks; ++j, ++c, ++i2) {
+            const bool more = j + 1 < a.chunks;
+            const int s1 = i1 % C::W1R, s2 = i2 % C::W2R;
+            if (more && !wait(&S.w1_full[s1], i1 / C::W1R)) return;
+            if (!wait(&S.w2_full[s2], i2 / C::W2R)) return;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                // h of this chunk is in shared memory, and D has been read
+                if (!wait(&S.h_ready[sub], c)) return;
+                if (j == 0 && k > 0 && !wait(&S.y_empty[sub], k - 1)) return;
+                tc_fence_after();
+                if (more) {
+                    product1(sub, s1);
+                    if (j + 2 == a.chunks) umma_commit(&S.x_empty[(ix + sub) % C::XR]);
+                    if (sub == 1) umma_commit(&S.w1_empty[s1]);
+                }
+                const uint32_t sh = smem_u32(S.h + sub * C::H_BYTES);
+                const uint32_t sw = smem_u32(S.w2 + s2 * C::W2_BYTES);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    umma_f16(tmem + sub * 128, sdesc_k_sw128(sh + ks * 32), sdesc_k_sw128(sw + ks * 32), idesc2,
+                             (j > 0 || ks > 0) ? 1u : 0u);
+                umma_commit(&S.h_free[sub]);
+                if (!more) umma_commit(&S.y_full[sub]);
+                if (sub == 1) umma_commit(&S.w2_empty[s2]);
+            }
+            if (more) ++i1;
+        }
+    }
+}
+
+template <int KC>
+__device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
+    using C = FusedCfg<KC>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int q = warp & 3, sub = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
+    const int m = q * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t d = tmem + lanes + 256 + sub * 128, y = tmem + lanes + sub * 128;
+    uint8_t* unit = S.h + sub * C::H_BYTES;
+    const bool issuer = lane == 0 && half == 0 && q == 0;
+    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    bool ok = true;
+    int c = 0, k = 0;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k) {
+        for (int j = 0; j < a.chunks; ++j, ++c) {
+            ok = ok && wait(&S.d_full[sub], c);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) continue;
+            tc_fence_after();
+            uint64_t h[2][8];
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+                const int col = half * 32 + cc * 16;
+                uint32_t rg[16], ru[16];
+                tmem_ld16(d + col, rg);
+                tmem_ld16(d + 64 + col, ru);
+                tmem_wait_ld_regs(rg);
+                tmem_wait_ld_regs(ru);
+                uint64_t u[8];
+                to_pairs(rg, h[cc]);
+                to_pairs(ru, u);
+                add_bias(a.b_gate, j * 64 + col, a.hidden, h[cc]);
+                add_bias(a.b_up, j * 64 + col, a.hidden, u);
+                gate_chunk(a.act, h[cc], u);
+                if (cc == 0) {
+                    // the products of the chunk before (and the store of the
+                    // tile before) have read the unit
+                    if (c > 0) ok = wait(&S.h_free[sub], c - 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                if (ok) put_unit(unit, m, col / 8, h[cc], a.bf16);
+            }
+            tc_fence_before();
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(&S.h_ready[sub]);
+        }
+        // the subtile's rows: through the h unit, 64 columns at a time
+        ok = ok && wait(&S.y_full[sub], k);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+#pragma unroll
+        for (int u0 = 0; u0 < C::CP; u0 += 64) {
+            if (u0 > 0) {
+                if (issuer) bulk_wait_read();
+                named_bar(1 + sub, 32 * kGroupWarps);
+            }
+            if (ok) {
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    const int col = half * 32 + cc * 16;
+                    uint32_t r[16];
+                    tmem_ld16(y + u0 + col, r);
+                    tmem_wait_ld_regs(r);
+                    if (u0 + 64 == C::CP && cc == 1) {
+                        tc_fence_before();
+                        warp_arrive(&S.y_empty[sub]);
+                    }
+                    uint64_t v[8];
+                    to_pairs(r, v);
+                    add_bias(a.b_down, u0 + col, a.c, v);
+                    put_unit(unit, m, col / 8, v, a.bf16);
+                }
+                fence_proxy_async();
+            }
+            named_bar(1 + sub, 32 * kGroupWarps);
+            if (ok && issuer) {
+                const int row0 = tile * 256 + sub * 128;
+                if (u0 < a.c && row0 < a.rows) tma_store_2d(&a.my, smem_u32(unit), u0, row0);
+                bulk_commit();
+            }
+        }
+        // the next tile's first h waits for the store to have read the unit
+        if (issuer) bulk_wait_read();
+        named_bar(1 + sub, 32 * kGroupWarps);
+    }
+    if (issuer) bulk_wait();
+}
+
+template <int KC>
+__global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_constant__ FusedArgs a) {
+    using C = FusedCfg<KC>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* p = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    FusedSmem S;
+    S.x = p;
+    p += C::XR * C::X_BYTES;
+    S.w1 = p;
+    p += C::W1R * C::W1_BYTES;
+    S.w2 = p;
+    p += C::W2R * C::W2_BYTES;
+    S.h = p;
+    p += 2 * C::H_BYTES;
+    S.x_full = reinterpret_cast<uint64_t*>(p);
+    S.x_empty = S.x_full + C::XR;
+    S.w1_full = S.x_empty + C::XR;
+    S.w1_empty = S.w1_full + C::W1R;
+    S.w2_full = S.w1_empty + C::W1R;
+    S.w2_empty = S.w2_full + C::W2R;
+    S.d_full = S.w2_empty + C::W2R;
+    S.h_ready = S.d_full + 2;
+    S.h_free = S.h_ready + 2;
+    S.y_full = S.h_free + 2;
+    S.y_empty = S.y_full + 2;
+    S.drained = S.y_empty + 2;
+    S.tmem = reinterpret_cast<uint32_t*>(S.drained + 1);
+    S.abort = reinterpret_cast<int*>(S.tmem + 1);
+    static_assert((2 * (C::XR + C::W1R + C::W2R) + 11) * 8 + 8 <= 512, "barriers fit");
+
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < 2 * (C::XR + C::W1R + C::W2R); ++s) mbar_init(&S.x_full[s], 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&S.d_full[s], 1);
+            mbar_init(&S.h_ready[s], kGroupWarps);
+            mbar_init(&S.h_free[s], 1);
+            mbar_init(&S.y_full[s], 1);
+            mbar_init(&S.y_empty[s], kGroupWarps);
+        }
+        mbar_init(S.drained, 1);
+        *S.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 2) {
+        tmem_alloc(S.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *S.tmem;
+
+    if (warp == 0) {
+        if ((threadIdx.x & 31) == 0) fused_producer<KC>(a, S);
+        __syncwarp();
+    } else if (warp == 1) {
+        if ((threadIdx.x & 31) == 0) {
+            fused_issuer<KC>(a, S, tmem);
+            if (*reinterpret_cast<volatile int*>(S.abort)) {
+                // MMAs sent before the abort may still write TMEM: a commit
+                // tracks them all; wait (bounded) before the columns go
+                umma_commit(S.drained);
+                (void)mbar_wait(S.drained, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        fused_epilogue<KC>(a, S, tmem);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int KC>
+cudaError_t launch_t(const FusedArgs& a, cudaStream_t st) {
+    using C = FusedCfg<KC>;
+    static std::mutex mu;
+    static int num_sms[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    int sms = 0;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!num_sms[dev]) {
+            e = cudaFuncSetAttribute(ffn_fused_kernel<KC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+            if (e != cudaSuccess) return e;
+            int count = 0;
+            e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+            if (e != cudaSuccess) return e;
+            num_sms[dev] = count;
+        }
+        sms = num_sms[dev];
+    }
+    ffn_fused_kernel<KC><<<std::min(a.tiles, sms), kThreads, C::SMEM, st>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_ffn_fused(const FfnShape& s, const void* x, const FfnWeights& w, void* y, uint32_t* status,
+                             cudaStream_t st) {
+    const bool bf = s.dtype == DT_BF16;
+    FusedArgs a{};
+    const int kc = s.c > 64 ? 2 : 1;
+    cudaError_t e = make_map_16bit(&a.mx, x, bf, s.n, s.c, 128);
+    if (e == cudaSuccess) e = make_map_16bit(&a.mg, w.w_gate, bf, s.hidden, s.c, 64);
+    if (e == cudaSuccess) e = make_map_16bit(&a.mu, w.w_up, bf, s.hidden, s.c, 64);
+    if (e == cudaSuccess) e = make_map_16bit(&a.md, w.w_down, bf, s.c, s.hidden, 64 * kc);
+    if (e == cudaSuccess) e = make_map_16bit(&a.my, y, bf, s.n, s.c, 128);
+    if (e != cudaSuccess) return e;
+    a.tiles = static_cast<int>((s.n + 255) / 256);
+    a.chunks = (s.hidden + 63) / 64;
+    a.rows = static_cast<int>(s.n);
+    a.c = s.c;
+    a.hidden = s.hidden;
+    a.b_gate = w.b_gate, a.b_up = w.b_up, a.b_down = w.b_down;
+    a.act = s.act;
+    a.bf16 = bf;
+    a.status = status;
+    return kc == 2 ? launch_t<2>(a, st) : launch_t<1>(a, st);
+}
+
+}  // namespace msc

@@ -210,38 +210,50 @@ __device__ void ffn_issuer(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tmem
     }
 }
 
-// N columns of a bias from col on (columns past the end: nothing added).
+// N accumulator registers as pairs.
 template <int N>
-__device__ __forceinline__ void add_bias(const float* b, int col, int cols, float (&v)[N]) {
+__device__ __forceinline__ void to_pairs(const uint32_t (&r)[N], uint64_t (&v)[N / 2]) {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) v[e] = pack2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+}
+
+// N pairs of a bias from col on (columns past the end: nothing added).
+template <int N>
+__device__ __forceinline__ void add_bias(const float* b, int col, int cols, uint64_t (&v)[N]) {
     if (!b) return;
 #pragma unroll
-    for (int e = 0; e < N; e += 4)
-        if (col + e < cols) {
-            const float4 t = __ldg(reinterpret_cast<const float4*>(b + col + e));
-            v[e] += t.x, v[e + 1] += t.y, v[e + 2] += t.z, v[e + 3] += t.w;
+    for (int e = 0; e < N; e += 2)
+        if (col + 2 * e < cols) {
+            const float4 t = __ldg(reinterpret_cast<const float4*>(b + col + 2 * e));
+            v[e] = add2(v[e], pack2(t.x, t.y));
+            v[e + 1] = add2(v[e + 1], pack2(t.z, t.w));
         }
 }
 
-// N values (a multiple of 8) as 16-bit 16-byte chunks of row m of a swizzled
+// N pairs (a multiple of 4) as 16-bit 16-byte chunks of row m of a swizzled
 // unit, from 16-byte chunk `chunk` on.
 template <int N>
-__device__ __forceinline__ void put_unit(uint8_t* unit, int m, int chunk, const float (&v)[N], int bf16) {
-    uint32_t w[N / 2];
+__device__ __forceinline__ void put_unit(uint8_t* unit, int m, int chunk, const uint64_t (&v)[N], int bf16) {
+    uint32_t w[N];
     if (bf16) {
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        for (int e = 0; e < N; ++e) {
+            float a, b;
+            unpack2(v[e], a, b);
+            const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
             w[e] = *reinterpret_cast<const uint32_t*>(&t);
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < N / 2; ++e) {
-            const __half2 t = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+        for (int e = 0; e < N; ++e) {
+            float a, b;
+            unpack2(v[e], a, b);
+            const __half2 t = __floats2half2_rn(a, b);
             w[e] = *reinterpret_cast<const uint32_t*>(&t);
         }
     }
 #pragma unroll
-    for (int k = 0; k < N / 8; ++k)
+    for (int k = 0; k < N / 4; ++k)
         *reinterpret_cast<uint4*>(unit + sw128_offset(m, chunk + k)) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 }
 
@@ -309,13 +321,10 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
                     tmem_wait_ld_regs(ru);
                     tmem_wait_ld_regs(rd);
                     if (cc == 1) release();
-                    float g[16], u[16], d[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        g[e] = __uint_as_float(rg[e]);
-                        u[e] = __uint_as_float(ru[e]);
-                        d[e] = __uint_as_float(rd[e]);
-                    }
+                    uint64_t g[8], u[8], d[8];
+                    to_pairs(rg, g);
+                    to_pairs(ru, u);
+                    to_pairs(rd, d);
                     add_bias(a.bias0, n0 + c0, cols, g);
                     add_bias(a.bias1, n0 + c0, cols, u);
                     gate_back_chunk(a.act, g, u, d);
@@ -324,12 +333,13 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
                     put_unit(S.out + 2 * C::UNIT_BYTES, m, c0 / 8, d, a.bf16);
                     if (a.bias_part) {
                         const bool live = m0 + m < rows;
+                        float fg[16], fu[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            g[e] = live ? g[e] : 0.f;
-                            u[e] = live ? u[e] : 0.f;
+                        for (int e = 0; e < 8; ++e) {
+                            unpack2(live ? g[e] : 0ull, fg[2 * e], fg[2 * e + 1]);
+                            unpack2(live ? u[e] : 0ull, fu[2 * e], fu[2 * e + 1]);
                         }
-                        const float sg = column_sums16(g, lane), su = column_sums16(u, lane);
+                        const float sg = column_sums16(fg, lane), su = column_sums16(fu, lane);
                         if (!(lane & 1)) {
                             S.red[(q * 2 + 0) * HT + c0 + (lane >> 1 & 1) + (lane >> 2 & 1) * 2 + (lane >> 3 & 1) * 4 +
                                   (lane >> 4) * 8] = sg;
@@ -374,7 +384,7 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
                 if (ok) {
 #pragma unroll
                     for (int cc = 0; cc < NC; cc += 32) {
-                        float v[32];
+                        uint64_t v[16];
                         if constexpr (MODE == FFN_HIDDEN) {
                             uint32_t rg[32], ru[32];
                             tmem_ld32(acc + u0 + cc, rg);
@@ -382,9 +392,9 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
                             tmem_wait_ld_regs(rg);
                             tmem_wait_ld_regs(ru);
                             if (last && cc + 32 == NC) release();
-                            float u[32];
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(rg[e]), u[e] = __uint_as_float(ru[e]);
+                            uint64_t u[16];
+                            to_pairs(rg, v);
+                            to_pairs(ru, u);
                             add_bias(a.bias0, n0 + u0 + cc, cols, v);
                             add_bias(a.bias1, n0 + u0 + cc, cols, u);
                             gate_chunk(a.act, v, u);
@@ -393,8 +403,7 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
                             tmem_ld32(acc + u0 + cc, r);
                             tmem_wait_ld_regs(r);
                             if (last && cc + 32 == NC) release();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
+                            to_pairs(r, v);
                             if (direct) {
                                 if (m0 + m < rows) {
                                     float* p = a.partial + t.split * a.partial_split + a.partial_prob[t.prob] +
@@ -402,7 +411,7 @@ __device__ void ffn_epilogue(const FfnGemmArgs& a, const FfnSmem& S, uint32_t tm
 #pragma unroll
                                     for (int e = 0; e < 32; e += 4)
                                         if (n0 + u0 + cc + e < cols)
-                                            *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                                            *reinterpret_cast<ulonglong2*>(p + e) = make_ulonglong2(v[e / 2], v[e / 2 + 1]);
                                 }
                                 continue;
                             }

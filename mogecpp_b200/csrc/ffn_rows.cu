@@ -101,11 +101,13 @@ __global__ void __launch_bounds__(32 * kWarps) rows_hidden_kernel(const void* x,
     const float bg = w.b_gate ? __ldg(w.b_gate + j) : 0.f, bu = w.b_up ? __ldg(w.b_up + j) : 0.f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-        float a[1] = {warp_total(g[r]) + bg};
-        const float b[1] = {warp_total(u[r]) + bu};
+        uint64_t a[1] = {both(warp_total(g[r]) + bg)};
+        const uint64_t b[1] = {both(warp_total(u[r]) + bu)};
         if (r < n && lane == r) {
             gate_chunk(act, a, b);
-            h[static_cast<int64_t>(r) * hidden + j] = a[0];
+            float v, same;
+            unpack2(a[0], v, same);
+            h[static_cast<int64_t>(r) * hidden + j] = v;
         }
     }
 }

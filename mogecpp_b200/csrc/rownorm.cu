@@ -163,7 +163,6 @@ __device__ __forceinline__ void store8(void* p, int64_t off, const uint64_t* v) 
     }
 }
 
-__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
 __device__ __forceinline__ float sum_pair(uint64_t v) {
     float a, b;
     unpack2(v, a, b);
