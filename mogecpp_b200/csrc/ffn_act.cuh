@@ -1,9 +1,10 @@
 // Activations of the gated feed-forward block and their derivatives, on
 // packed f32 pairs.
 //
-// The special-function unit would bound the epilogues (one exp2 and one
-// reciprocal an element, 16 a cycle and SM), so that only the exp2 runs
-// there; the reciprocal is Newton's method on packed fused multiply-adds.
+// The special-function unit bounds these epilogues first (16 results a cycle
+// and SM): an exp2 and a reciprocal an element would take it longer than the
+// tensor cores take for the products at 64 or 128 channels.  So two elements
+// share one reciprocal.
 #pragma once
 
 #include "common.cuh"
@@ -26,29 +27,21 @@ __device__ __forceinline__ uint64_t min2(uint64_t v, float m) {
     return pack2(fminf(a, m), fminf(b, m));
 }
 
-// 1 / d from nd = -d, 1 <= d <= 2^101.  A float's bits are, up to a linear
-// interpolation within each octave, 2^23 times its logarithm, so that a
-// constant minus them is a first reciprocal y; the constant (found by search
-// over an octave) leaves |r| = |1 - d y| <= 0.0506.  One third-order step
-// y (1 + r + r^2) leaves r^3 = 1.3e-4, one Newton step its square, 1.7e-8.
-__device__ __forceinline__ uint64_t reciprocal2(uint64_t nd) {
-    constexpr uint32_t kSeed = 0x7ef31000u + 0x80000000u;  // the sign of nd cancels
-    const uint64_t one = both(1.0f);
-    float a, b;
-    unpack2(nd, a, b);
-    uint64_t y = pack2(__uint_as_float(kSeed - __float_as_uint(a)), __uint_as_float(kSeed - __float_as_uint(b)));
-    uint64_t r = fma2(nd, y, one);
-    y = fma2(y, fma2(r, r, r), y);
-    r = fma2(nd, y, one);
-    return fma2(y, r, y);
+// 1 / d of both lanes from the reciprocal of their product, r = 1 / (d0 d1):
+// 1 / d0 = r d1, 1 / d1 = r d0 (a few ulp).  1 <= d <= 2^63, so that the
+// product stays finite.
+__device__ __forceinline__ uint64_t reciprocal2(uint64_t d) {
+    float a, b, r;
+    unpack2(d, a, b);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+    return mul2(both(r), pack2(b, a));
 }
 
-// sigma(v) = 1 / (1 + 2^(-v log2 e)).  The exponent is held at 100, where
-// sigma is 2^-100 in place of less: nothing next to the smallest value that
-// a 16-bit result distinguishes from zero at any magnitude of v.
+// sigma(v) = 1 / (1 + 2^(-v log2 e)).  The exponent is held at 62, where
+// sigma is 2^-62 in place of less: v sigma(v) is then off by |v| 2^-62 at
+// most.
 __device__ __forceinline__ uint64_t sigmoid2(uint64_t v) {
-    const uint64_t e = exp2_2(min2(mul2(v, both(-1.4426950408889634f)), 100.0f));
-    return reciprocal2(fma2(e, both(-1.0f), both(-1.0f)));
+    return reciprocal2(add2(exp2_2(min2(mul2(v, both(-1.4426950408889634f)), 62.0f)), both(1.0f)));
 }
 
 // GELU's tanh form as g sigma(2 z), z = sqrt(2/pi) (g + 0.044715 g^3): the
@@ -63,18 +56,15 @@ constexpr float kGelu1 = 0.07135481282553484f;  // 2 sqrt(2/pi) 0.044715
 __device__ __forceinline__ uint64_t normal_cdf2(uint64_t g, uint64_t& gauss) {
     constexpr uint64_t kSigns = 0x8000000080000000ull;
     const uint64_t z = min2(g & ~kSigns, 20.0f);
-    const uint64_t t = reciprocal2(fma2(z, both(-0.3275911f * 0.7071067811865476f), both(-1.0f)));
+    const uint64_t t = reciprocal2(fma2(z, both(0.3275911f * 0.7071067811865476f), both(1.0f)));
     gauss = exp2_2(mul2(mul2(z, z), both(-0.7213475204444817f)));  // -log2(e) / 2
-    // the polynomial's coefficients halved: Phi(-|g|) = erfc / 2
-    uint64_t p = fma2(t, both(0.5f * 1.061405429f), both(-0.5f * 1.453152027f));
-    p = fma2(t, p, both(0.5f * 1.421413741f));
-    p = fma2(t, p, both(-0.5f * 0.284496736f));
-    p = fma2(t, p, both(0.5f * 0.254829592f));
-    p = mul2(mul2(t, p), gauss);
-    float p0, p1, g0, g1;
-    unpack2(p, p0, p1);
-    unpack2(g, g0, g1);
-    return pack2(g0 > 0.f ? 1.f - p0 : p0, g1 > 0.f ? 1.f - p1 : p1);
+    // the polynomial's coefficients halved and negated: Phi(|g|) - 1/2 = 1/2 - erfc / 2
+    uint64_t p = fma2(t, both(-0.5f * 1.061405429f), both(0.5f * 1.453152027f));
+    p = fma2(t, p, both(-0.5f * 1.421413741f));
+    p = fma2(t, p, both(0.5f * 0.284496736f));
+    p = fma2(t, p, both(-0.5f * 0.254829592f));
+    p = fma2(mul2(t, p), gauss, both(0.5f));
+    return add2((p & ~kSigns) | (g & kSigns), both(0.5f));
 }
 
 template <int ACT>

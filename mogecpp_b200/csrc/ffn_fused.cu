@@ -9,13 +9,15 @@
 //   h = act(D_g + bg) * (D_u + bu)  (epilogue warps -> shared memory, 16 bits)
 //   Y += h Wd[:, chunk]^T           (TMEM, 128 rows x c columns, K = 64)
 // The weights stream through shared memory once per 256 rows (they stay in
-// L2).  The two subtiles run half a chunk apart: while the epilogue warps of
-// one turn D into h, the tensor core works on the other, and each subtile's
-// next D is issued before its Y so that its epilogue can go on at once.
+// L2).  The epilogue is the long pole (a gated activation an element), so it
+// never waits for the tensor core: its warps take a whole chunk of D into
+// registers and release D before they compute, and the next chunk's D is
+// there when they are done.  The two products have an issuing warp each, so
+// that neither waits for the other's operands.
 //
-// TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 MMA
-// issuer, 2 TMEM allocation, 4-19 epilogue (8 per subtile: lane quarter x
-// half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
+// TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 and 2
+// MMA issuers (D, Y), 3 TMEM allocation, 4-19 epilogue (8 per subtile: lane
+// quarter x half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
 #include "ffn_fused.h"
 
 #include "common.cuh"
@@ -63,7 +65,7 @@ struct alignas(64) FusedArgs {
 struct FusedSmem {
     uint8_t *x, *w1, *w2, *h;
     uint64_t *x_full, *x_empty, *w1_full, *w1_empty, *w2_full, *w2_empty;
-    uint64_t *d_full, *h_ready, *h_free, *y_full, *y_empty, *drained;  // per subtile
+    uint64_t *d_full, *d_free, *h_ready, *h_free, *y_full, *y_empty, *drained;  // per subtile / issuer
     uint32_t* tmem;
     int* abort;
 };
@@ -129,62 +131,64 @@ __device__ void fused_producer(const FusedArgs& a, const FusedSmem& S) {
     }
 }
 
+// D = x [Wg | Wu]^T of every chunk, subtiles in turn.
 template <int KC>
-__device__ void fused_issuer(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
+__device__ void fused_issue_d(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
     using C = FusedCfg<KC>;
-    const uint32_t fmt = a.bf16 ? 1u : 0u;
-    const uint32_t idesc1 = idesc_f16(128, 128, fmt), idesc2 = idesc_f16(128, C::CP, fmt);
-    int ix = 0, i1 = 0, i2 = 0, c = 0, k = 0;  // x slots, weight stages, chunks and tiles so far
+    const uint32_t idesc = idesc_f16(128, 128, a.bf16 ? 1u : 0u);
+    int ix = 0, c = 0;  // x slots, chunks so far
     auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k, ix += 2) {
-        auto product1 = [&](int sub, int stage) {
-            const uint32_t sx = smem_u32(S.x + ((ix + sub) % C::XR) * C::X_BYTES);
-            const uint32_t sw = smem_u32(S.w1 + stage * C::W1_BYTES);
-#pragma unroll
-            for (int ks = 0; ks < KC * 4; ++ks) {
-                const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
-                umma_f16(tmem + 256 + sub * 128, sdesc_k_sw128(sx + off), sdesc_k_sw128(sw + off), idesc1, ks > 0 ? 1u : 0u);
-            }
-            umma_commit(&S.d_full[sub]);
-        };
-        // first chunk of both subtiles
-        if (!wait(&S.w1_full[i1 % C::W1R], i1 / C::W1R)) return;
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            if (!wait(&S.x_full[(ix + sub) % C::XR], (ix + sub) / C::XR)) return;
-            tc_fence_after();
-            product1(sub, i1 % C::W1R);
-            if (a.chunks == 1) umma_commit(&S.x_empty[(ix + sub) % C::XR]);
-        }
-        umma_commit(&S.w1_empty[i1 % C::W1R]);
-        ++i1;
-        for (int j = 0; j < a.chunks; ++j, ++c, ++i2) {
-            const bool more = j + 1 < a.chunks;
-            const int s1 = i1 % C::W1R, s2 = i2 % C::W2R;
-            if (more && !wait(&S.w1_full[s1], i1 / C::W1R)) return;
-            if (!wait(&S.w2_full[s2], i2 / C::W2R)) return;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ix += 2) {
+        for (int j = 0; j < a.chunks; ++j, ++c) {
+            const int s = c % C::W1R;
+            if (!wait(&S.w1_full[s], c / C::W1R)) return;
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-                // h of this chunk is in shared memory, and D has been read
+                const int xs = (ix + sub) % C::XR;
+                if (j == 0 && !wait(&S.x_full[xs], (ix + sub) / C::XR)) return;
+                if (c > 0 && !wait(&S.d_free[sub], c - 1)) return;
+                tc_fence_after();
+                const uint32_t sx = smem_u32(S.x + xs * C::X_BYTES);
+                const uint32_t sw = smem_u32(S.w1 + s * C::W1_BYTES);
+#pragma unroll
+                for (int ks = 0; ks < KC * 4; ++ks) {
+                    const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
+                    umma_f16(tmem + 256 + sub * 128, sdesc_k_sw128(sx + off), sdesc_k_sw128(sw + off), idesc, ks > 0 ? 1u : 0u);
+                }
+                umma_commit(&S.d_full[sub]);
+                if (j + 1 == a.chunks) umma_commit(&S.x_empty[xs]);
+            }
+            umma_commit(&S.w1_empty[s]);
+        }
+    }
+}
+
+// Y += h Wd^T of every chunk, subtiles in turn.
+template <int KC>
+__device__ void fused_issue_y(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
+    using C = FusedCfg<KC>;
+    const uint32_t idesc = idesc_f16(128, C::CP, a.bf16 ? 1u : 0u);
+    int c = 0, k = 0;  // chunks, tiles so far
+    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k) {
+        for (int j = 0; j < a.chunks; ++j, ++c) {
+            const int s = c % C::W2R;
+            if (!wait(&S.w2_full[s], c / C::W2R)) return;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
                 if (!wait(&S.h_ready[sub], c)) return;
                 if (j == 0 && k > 0 && !wait(&S.y_empty[sub], k - 1)) return;
                 tc_fence_after();
-                if (more) {
-                    product1(sub, s1);
-                    if (j + 2 == a.chunks) umma_commit(&S.x_empty[(ix + sub) % C::XR]);
-                    if (sub == 1) umma_commit(&S.w1_empty[s1]);
-                }
                 const uint32_t sh = smem_u32(S.h + sub * C::H_BYTES);
-                const uint32_t sw = smem_u32(S.w2 + s2 * C::W2_BYTES);
+                const uint32_t sw = smem_u32(S.w2 + s * C::W2_BYTES);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
-                    umma_f16(tmem + sub * 128, sdesc_k_sw128(sh + ks * 32), sdesc_k_sw128(sw + ks * 32), idesc2,
+                    umma_f16(tmem + sub * 128, sdesc_k_sw128(sh + ks * 32), sdesc_k_sw128(sw + ks * 32), idesc,
                              (j > 0 || ks > 0) ? 1u : 0u);
                 umma_commit(&S.h_free[sub]);
-                if (!more) umma_commit(&S.y_full[sub]);
-                if (sub == 1) umma_commit(&S.w2_empty[s2]);
+                if (j + 1 == a.chunks) umma_commit(&S.y_full[sub]);
             }
-            if (more) ++i1;
+            umma_commit(&S.w2_empty[s]);
         }
     }
 }
@@ -208,33 +212,29 @@ __device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t 
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             tc_fence_after();
-            uint64_t h[2][8];
-#pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-                const int col = half * 32 + cc * 16;
-                uint32_t rg[16], ru[16];
-                tmem_ld16(d + col, rg);
-                tmem_ld16(d + 64 + col, ru);
+            const int col = half * 32;
+            uint64_t g[16], u[16];
+            {
+                uint32_t rg[32], ru[32];
+                tmem_ld32(d + col, rg);
+                tmem_ld32(d + 64 + col, ru);
                 tmem_wait_ld_regs(rg);
                 tmem_wait_ld_regs(ru);
-                uint64_t u[8];
-                to_pairs(rg, h[cc]);
+                tc_fence_before();
+                warp_arrive(&S.d_free[sub]);
+                to_pairs(rg, g);
                 to_pairs(ru, u);
-                add_bias(a.b_gate, j * 64 + col, a.hidden, h[cc]);
-                add_bias(a.b_up, j * 64 + col, a.hidden, u);
-                gate_chunk(a.act, h[cc], u);
-                if (cc == 0) {
-                    // the products of the chunk before (and the store of the
-                    // tile before) have read the unit
-                    if (c > 0) ok = wait(&S.h_free[sub], c - 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                }
-                if (ok) put_unit(unit, m, col / 8, h[cc], a.bf16);
             }
-            tc_fence_before();
+            add_bias(a.b_gate, j * 64 + col, a.hidden, g);
+            add_bias(a.b_up, j * 64 + col, a.hidden, u);
+            gate_chunk(a.act, g, u);
+            // the product of the chunk before has read the unit
+            if (c > 0) ok = wait(&S.h_free[sub], c - 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) continue;
+            put_unit(unit, m, col / 8, g, a.bf16);
             fence_proxy_async();
-            __syncwarp();
-            if (lane == 0 && ok) mbar_arrive(&S.h_ready[sub]);
+            warp_arrive(&S.h_ready[sub]);
         }
         // the subtile's rows: through the h unit, 64 columns at a time
         ok = ok && wait(&S.y_full[sub], k);
@@ -299,30 +299,32 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     S.w2_full = S.w1_empty + C::W1R;
     S.w2_empty = S.w2_full + C::W2R;
     S.d_full = S.w2_empty + C::W2R;
-    S.h_ready = S.d_full + 2;
+    S.d_free = S.d_full + 2;
+    S.h_ready = S.d_free + 2;
     S.h_free = S.h_ready + 2;
     S.y_full = S.h_free + 2;
     S.y_empty = S.y_full + 2;
     S.drained = S.y_empty + 2;
-    S.tmem = reinterpret_cast<uint32_t*>(S.drained + 1);
+    S.tmem = reinterpret_cast<uint32_t*>(S.drained + 2);
     S.abort = reinterpret_cast<int*>(S.tmem + 1);
-    static_assert((2 * (C::XR + C::W1R + C::W2R) + 11) * 8 + 8 <= 512, "barriers fit");
+    static_assert((2 * (C::XR + C::W1R + C::W2R) + 14) * 8 + 8 <= 512, "barriers fit");
 
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2 * (C::XR + C::W1R + C::W2R); ++s) mbar_init(&S.x_full[s], 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&S.d_full[s], 1);
+            mbar_init(&S.d_free[s], kGroupWarps);
             mbar_init(&S.h_ready[s], kGroupWarps);
             mbar_init(&S.h_free[s], 1);
             mbar_init(&S.y_full[s], 1);
             mbar_init(&S.y_empty[s], kGroupWarps);
+            mbar_init(&S.drained[s], 1);
         }
-        mbar_init(S.drained, 1);
         *S.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 2) {
+    if (warp == 3) {
         tmem_alloc(S.tmem, 512);
         tmem_relinquish();
     }
@@ -334,15 +336,12 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     if (warp == 0) {
         if ((threadIdx.x & 31) == 0) fused_producer<KC>(a, S);
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp <= 2) {
         if ((threadIdx.x & 31) == 0) {
-            fused_issuer<KC>(a, S, tmem);
-            if (*reinterpret_cast<volatile int*>(S.abort)) {
-                // MMAs sent before the abort may still write TMEM: a commit
-                // tracks them all; wait (bounded) before the columns go
-                umma_commit(S.drained);
-                (void)mbar_wait(S.drained, 0);
-            }
+            if (warp == 1)
+                fused_issue_d<KC>(a, S, tmem);
+            else
+                fused_issue_y<KC>(a, S, tmem);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -350,7 +349,16 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 2) {
+    if (*reinterpret_cast<volatile int*>(S.abort)) {
+        // MMAs sent before the abort may still write TMEM: a commit tracks an
+        // issuer's; wait (bounded) before the columns go
+        if ((warp == 1 || warp == 2) && (threadIdx.x & 31) == 0) {
+            umma_commit(&S.drained[warp - 1]);
+            (void)mbar_wait(&S.drained[warp - 1], 0);
+        }
+        __syncthreads();
+    }
+    if (warp == 3) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

@@ -482,21 +482,22 @@ __global__ void __launch_bounds__(kFfnThreads, 1) ffn_gemm_kernel(const __grid_c
         if ((threadIdx.x & 31) == 0) ffn_producer<MODE, HT>(a, S);
         __syncwarp();
     } else if (warp == 1) {
-        if ((threadIdx.x & 31) == 0) {
-            ffn_issuer<MODE, HT>(a, S, tmem);
-            if (*reinterpret_cast<volatile int*>(S.abort)) {
-                // MMAs sent before the abort may still write TMEM: a commit
-                // tracks them all; wait (bounded) before the columns go
-                umma_commit(S.drained);
-                (void)mbar_wait(S.drained, 0);
-            }
-        }
+        if ((threadIdx.x & 31) == 0) ffn_issuer<MODE, HT>(a, S, tmem);
         __syncwarp();
     } else if (warp >= 4) {
         ffn_epilogue<MODE, HT>(a, S, tmem);
     }
     tc_fence_before();
     __syncthreads();
+    if (*reinterpret_cast<volatile int*>(S.abort)) {
+        // MMAs sent before the abort may still write TMEM: a commit tracks
+        // them all; wait (bounded) before the columns go
+        if (threadIdx.x == 32) {
+            umma_commit(S.drained);
+            (void)mbar_wait(S.drained, 0);
+        }
+        __syncthreads();
+    }
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, C::TMEM_COLS);
