@@ -48,13 +48,21 @@ constexpr int kSms = 148;  // B200; fixed, so that the split of a sum and the wo
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Column tile of a product with `cols` output columns: the widest that still
+// Tile of a product with `cols` output columns: pairs of CTAs on 256 rows
+// where every pair of SMs gets one, else the widest column tile that still
 // gives every SM a tile (wider tiles read less shared memory per product;
 // narrower ones spread few rows over more SMs).
-int col_tile(int64_t m_tiles, int cols) {
-    for (int ht = 256; ht > 64; ht /= 2)
-        if (cols > ht / 2 && m_tiles * cdiv(cols, ht) >= kSms) return ht;
-    return 64;
+struct TilePlan {
+    int ht, cg;
+};
+TilePlan tile_plan(int64_t rows, int cols) {
+    const int64_t m = cdiv(rows, 128), pairs = cdiv(rows, 256);
+    for (int ht = 256; ht > 64; ht /= 2) {
+        if (cols <= ht / 2) continue;
+        if (pairs * cdiv(cols, ht) >= kSms / 2) return {ht, 2};
+        if (m * cdiv(cols, ht) >= kSms) return {ht, 1};
+    }
+    return {64, 1};
 }
 
 // Splits of a K of `ksteps` steps when `tiles` output tiles leave SMs idle.
@@ -67,25 +75,31 @@ int k_splits(int64_t tiles, int ksteps, int min_steps, int* ksplit) {
 }
 
 struct ProjPlan {
-    int ht, splits, ksplit;
+    int ht, cg, splits, ksplit;
 };
 ProjPlan proj_plan(int64_t n, int cols, int ksteps) {
-    ProjPlan p{};
-    const int64_t m = cdiv(n, 128);
-    p.ht = col_tile(m, cols);
-    p.splits = k_splits(m * cdiv(cols, p.ht), ksteps, 4, &p.ksplit);
+    const TilePlan t = tile_plan(n, cols);
+    ProjPlan p{t.ht, t.cg, 1, ksteps};
+    if (t.cg == 1) p.splits = k_splits(cdiv(n, 128) * cdiv(cols, p.ht), ksteps, 4, &p.ksplit);
     return p;
 }
 
 struct DwPlan {
-    int ht, splits, ksplit, tiles;
+    int ht, cg, splits, ksplit, tiles;
 };
 DwPlan dw_plan(int64_t n, int c, int hidden) {
     DwPlan p{};
     p.ht = c > 128 ? 256 : (c > 64 ? 128 : 64);
-    p.tiles = static_cast<int>(2 * cdiv(hidden, 128) * cdiv(c, p.ht) + cdiv(c, 128) * cdiv(hidden, p.ht));
+    p.cg = 1;
+    auto tiles = [&](int cg) {
+        return static_cast<int>(2 * cdiv(hidden, 128 * cg) * cdiv(c, p.ht) + cdiv(c, 128 * cg) * cdiv(hidden, p.ht));
+    };
+    if (p.ht == 256 && tiles(2) >= kSms / 2) p.cg = 2;
+    p.tiles = tiles(p.cg);
     const int ksteps = static_cast<int>(cdiv(n, 64));
-    p.splits = k_splits(p.tiles, ksteps, 4, &p.ksplit);
+    p.splits = 1;
+    p.ksplit = std::max(ksteps, 1);
+    if (p.cg == 1) p.splits = k_splits(p.tiles, ksteps, 4, &p.ksplit);
     // no sum in one accumulator runs over more than 32768 rows: the tensor
     // core's fp32 accumulator truncates, a drift that grows with the chain
     if (p.ksplit > 512) {
@@ -95,52 +109,68 @@ DwPlan dw_plan(int64_t n, int c, int hidden) {
     return p;
 }
 
-template <int MODE, int HT>
+template <int MODE, int HT, int CG>
 cudaError_t launch_gemm_t(const FfnGemmArgs& a, cudaStream_t st) {
-    using C = FfnCfg<MODE, HT>;
-    auto kern = ffn_gemm_kernel<MODE, HT>;
+    using C = FfnCfg<MODE, HT, CG>;
+    auto kern = ffn_gemm_kernel<MODE, HT, CG>;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = CG;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = CG == 2 ? 1 : 0;
+    // per device and instantiation: the shared-memory opt-in and the CTAs
+    // (pairs) that run at once, set up once under a lock
     static std::mutex mu;
-    static int num_sms[64] = {0};
+    static int at_once[64] = {0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    int sms = 0;
+    int running = 0;
     {
         std::lock_guard<std::mutex> lk(mu);
-        if (!num_sms[dev]) {
+        if (!at_once[dev]) {
             e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
             if (e != cudaSuccess) return e;
             int count = 0;
-            e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+            if constexpr (CG == 2) {
+                cfg.gridDim = dim3(CG);
+                e = cudaOccupancyMaxActiveClusters(&count, kern, &cfg);
+            } else {
+                e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+            }
             if (e != cudaSuccess) return e;
-            num_sms[dev] = count;
+            if (count < 1) return cudaErrorInvalidConfiguration;
+            at_once[dev] = count;
         }
-        sms = num_sms[dev];
+        running = at_once[dev];
     }
-    const int total = a.tiles * a.splits;
-    kern<<<std::min(total, sms), kFfnThreads, C::SMEM, st>>>(a);
-    return cudaGetLastError();
+    cfg.gridDim = dim3(static_cast<unsigned>(CG * std::min(a.tiles * a.splits, running)));
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int MODE>
-cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, cudaStream_t st) {
-    if constexpr (MODE == FFN_HBACK) return launch_gemm_t<MODE, 64>(a, st);
-    if constexpr (MODE == FFN_HIDDEN) {
-        if (ht == 128) return launch_gemm_t<MODE, 128>(a, st);
-        return launch_gemm_t<MODE, 64>(a, st);
+cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, int cg, cudaStream_t st) {
+    if constexpr (MODE == FFN_HBACK) {
+        return cg == 2 ? launch_gemm_t<MODE, 128, 2>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
+    } else if constexpr (MODE == FFN_HIDDEN) {
+        if (cg == 2) return launch_gemm_t<MODE, 128, 2>(a, st);
+        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
+    } else {
+        if (cg == 2) return ht == 256 ? launch_gemm_t<MODE, 256, 2>(a, st) : launch_gemm_t<MODE, 128, 2>(a, st);
+        if (ht == 256) return launch_gemm_t<MODE, 256, 1>(a, st);
+        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
     }
-    if constexpr (MODE == FFN_PROJ || MODE == FFN_DX || MODE == FFN_DW) {
-        if (ht == 256) return launch_gemm_t<MODE, 256>(a, st);
-        if (ht == 128) return launch_gemm_t<MODE, 128>(a, st);
-        return launch_gemm_t<MODE, 64>(a, st);
-    }
-    return cudaErrorInvalidValue;
 }
 
-void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht) {
+void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht, int cg) {
     a.nprob = 1;
-    a.m_tiles[0] = static_cast<int>(cdiv(rows, 128));
+    a.m_tiles[0] = static_cast<int>(cdiv(rows, 128 * cg));
     a.n_tiles[0] = static_cast<int>(cdiv(cols, ht));
     a.rows[0] = static_cast<int>(rows);
     a.cols[0] = cols;
@@ -330,24 +360,26 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
     const int64_t m = cdiv(s.n, 128);
     {
         FfnGemmArgs a{};
-        const int ht = m * cdiv(s.hidden, 128) >= kSms ? 128 : 64;
+        // pairs on 256 rows x 128 hidden units, as tile_plan
+        const int cg = cdiv(s.n, 256) * cdiv(s.hidden, 128) >= kSms / 2 ? 2 : 1;
+        const int ht = cg == 2 || m * cdiv(s.hidden, 128) >= kSms ? 128 : 64;
         MSC_TRY(make_map_16bit(&a.ma[0], x, bf, s.n, s.c, 128));
         MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, ht));
         MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, ht));
         MSC_TRY(make_map_16bit(&a.mo[0], h, bf, s.n, s.hidden, 128));
         a.ksteps[0] = static_cast<int>(cdiv(s.c, 64));
-        one_problem(a, s.n, s.hidden, ht);
+        one_problem(a, s.n, s.hidden, ht, cg);
         a.bias0 = w.b_gate, a.bias1 = w.b_up;
         a.act = s.act, a.bf16 = bf, a.status = status;
-        MSC_TRY(launch_gemm<FFN_HIDDEN>(a, ht, st));
+        MSC_TRY(launch_gemm<FFN_HIDDEN>(a, ht, cg, st));
     }
     FfnGemmArgs a{};
     a.ksteps[0] = static_cast<int>(cdiv(s.hidden, 64));
     const ProjPlan p = proj_plan(s.n, s.c, a.ksteps[0]);
     MSC_TRY(make_map_16bit(&a.ma[0], h, bf, s.n, s.hidden, 128));
-    MSC_TRY(make_map_16bit(&a.mb[0], w.w_down, bf, s.c, s.hidden, p.ht));
+    MSC_TRY(make_map_16bit(&a.mb[0], w.w_down, bf, s.c, s.hidden, p.ht / p.cg));
     MSC_TRY(make_map_16bit(&a.mo[0], y, bf, s.n, s.c, 128));
-    one_problem(a, s.n, s.c, p.ht);
+    one_problem(a, s.n, s.c, p.ht, p.cg);
     a.splits = p.splits, a.ksplit = p.ksplit;
     a.bias0 = w.b_down;
     a.bf16 = bf, a.status = status;
@@ -355,7 +387,7 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
         a.partial = reinterpret_cast<float*>(base + o.part);
         a.partial_split = s.n * s.c;
     }
-    MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, st));
+    MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, p.cg, st));
     if (p.splits > 1) {
         const int64_t e = s.n * s.c;
         const SplitSumArgs r{a.partial, e, p.splits, {y, nullptr, nullptr}, {0, e, e, e}, w.b_down, s.c, bf};
@@ -389,20 +421,22 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
     const int64_t m = cdiv(s.n, 128);
     {
         FfnGemmArgs a{};
-        MSC_TRY(make_map_16bit(&a.ma[0], x, bf, s.n, s.c, 128));
-        MSC_TRY(make_map_16bit(&a.ma[1], dy, bf, s.n, s.c, 128));
-        MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, 64));
-        MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, 64));
+        const int cg = cdiv(s.n, 256) * cdiv(s.hidden, 128) >= kSms / 2 ? 2 : 1;
+        const int ht = 64 * cg;
+        MSC_TRY(make_map_16bit(&a.ma[0], dy, bf, s.n, s.c, 128));
+        MSC_TRY(make_map_16bit(&a.ma[1], x, bf, s.n, s.c, 128));
+        MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, ht));
+        MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, ht));
         MSC_TRY(make_map_16bit(&a.mb[2], w.w_down, bf, s.c, s.hidden, 64));
         MSC_TRY(make_map_16bit(&a.mo[0], dg, bf, s.n, s.hidden, 128));
         MSC_TRY(make_map_16bit(&a.mo[1], du, bf, s.n, s.hidden, 128));
         MSC_TRY(make_map_16bit(&a.mo[2], h, bf, s.n, s.hidden, 128));
         a.ksteps[0] = a.ksteps[1] = kc;
-        one_problem(a, s.n, s.hidden, 64);
+        one_problem(a, s.n, s.hidden, ht, cg);
         a.bias0 = w.b_gate, a.bias1 = w.b_up;
         if (g.b_gate || g.b_up) a.bias_part = reinterpret_cast<float*>(base + o.bias);
         a.act = s.act, a.bf16 = bf, a.status = status;
-        MSC_TRY(launch_gemm<FFN_HBACK>(a, 64, st));
+        MSC_TRY(launch_gemm<FFN_HBACK>(a, ht, cg, st));
         if (a.bias_part) MSC_TRY(launch_column_total(a.bias_part, m, 2 * s.hidden, s.hidden, g.b_gate, g.b_up, st));
     }
     if (g.b_down) {
@@ -422,14 +456,14 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
         MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, 64));
         MSC_TRY(make_map_16bit(&a.mo[0], g.dx, bf, s.n, s.c, 128));
         a.ksteps[0] = a.ksteps[1] = kh;
-        one_problem(a, s.n, s.c, p.ht);
+        one_problem(a, s.n, s.c, p.ht, p.cg);
         a.splits = p.splits, a.ksplit = p.ksplit;
         a.bf16 = bf, a.status = status;
         if (p.splits > 1) {
             a.partial = part;
             a.partial_split = s.n * s.c;
         }
-        MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, st));
+        MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, p.cg, st));
         if (p.splits > 1) {
             const int64_t e = s.n * s.c;
             const SplitSumArgs r{part, e, p.splits, {g.dx, nullptr, nullptr}, {0, e, e, e}, nullptr, s.c, bf};
@@ -448,7 +482,7 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
             MSC_TRY(make_map_16bit(&a.ma[i], am[i], bf, s.n, rows, 64));
             MSC_TRY(make_map_16bit(&a.mb[i], bm[i], bf, s.n, cols, 64));
             MSC_TRY(make_map_16bit(&a.mo[i], om[i], bf, rows, cols, 128));
-            a.m_tiles[i] = static_cast<int>(cdiv(rows, 128));
+            a.m_tiles[i] = static_cast<int>(cdiv(rows, 128 * p.cg));
             a.n_tiles[i] = static_cast<int>(cdiv(cols, p.ht));
             a.rows[i] = rows, a.cols[i] = cols;
             a.partial_prob[i] = i * ch;
@@ -461,7 +495,7 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
             a.partial = part;
             a.partial_split = 3 * ch;
         }
-        MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, st));
+        MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, p.cg, st));
         if (p.splits > 1) {
             const SplitSumArgs r{part, 3 * ch, p.splits, {om[0], om[1], om[2]}, {0, ch, 2 * ch, 3 * ch}, nullptr, s.c, bf};
             MSC_TRY(launch_split_sum(r, st));

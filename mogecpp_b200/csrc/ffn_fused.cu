@@ -9,15 +9,16 @@
 //   h = act(D_g + bg) * (D_u + bu)  (epilogue warps -> shared memory, 16 bits)
 //   Y += h Wd[:, chunk]^T           (TMEM, 128 rows x c columns, K = 64)
 // The weights stream through shared memory once per 256 rows (they stay in
-// L2).  The epilogue is the long pole (a gated activation an element), so it
-// never waits for the tensor core: its warps take a whole chunk of D into
-// registers and release D before they compute, and the next chunk's D is
-// there when they are done.  The two products have an issuing warp each, so
-// that neither waits for the other's operands.
+// L2).  The epilogue is the long pole (a gated activation an element, bound by
+// the special-function unit), so that it is kept from waiting: three groups
+// of warps take the (chunk, subtile) items in turn, each takes its D into
+// registers and releases it before it is done computing, and the next D is
+// there when a group comes back.  The two products have an issuing warp each,
+// so that neither waits for the other's operands, and a third warp stores.
 //
 // TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 and 2
-// MMA issuers (D, Y), 3 TMEM allocation, 4-19 epilogue (8 per subtile: lane
-// quarter x half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
+// MMA issuers (D, Y), 3 TMEM allocation and stores, 4-27 epilogue (8 per
+// group: lane quarter x half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
 #include "ffn_fused.h"
 
 #include "common.cuh"
@@ -33,21 +34,25 @@
 namespace msc {
 namespace {
 
-constexpr int kThreads = 640;
-constexpr int kGroupWarps = 8;  // epilogue warps of a subtile
+constexpr int kGroups = 3;
+constexpr int kGroupWarps = 8;
+constexpr int kThreads = 32 * (4 + kGroups * kGroupWarps);
 
 // KC: 64-channel blocks of a row (c padded with zeros by the copies).
 template <int KC>
 struct FusedCfg {
     static constexpr int XR = KC == 1 ? 4 : 2;   // x subtile slots
-    static constexpr int W1R = KC == 1 ? 4 : 3;  // gate and up weight stages
+    static constexpr int W1R = KC == 1 ? 4 : 2;  // gate and up weight stages
     static constexpr int W2R = KC == 1 ? 4 : 2;  // down weight stages
     static constexpr int X_BYTES = KC * 128 * 128;
     static constexpr int W1_BYTES = KC * 128 * 128;  // per 64-channel block: 64 gate rows, then 64 up rows
     static constexpr int W2_BYTES = KC * 64 * 128;   // c rows of 64 hidden units
     static constexpr int H_BYTES = 128 * 128;
     static constexpr int CP = KC * 64;  // padded channels
-    static constexpr int SMEM = 1024 + XR * X_BYTES + W1R * W1_BYTES + W2R * W2_BYTES + 2 * H_BYTES + 512;
+    // a subtile's h unit, which also takes the last 64 columns of its y on
+    // their way out, and a unit for each 64 columns before
+    static constexpr int UNITS = KC;
+    static constexpr int SMEM = 1024 + XR * X_BYTES + W1R * W1_BYTES + W2R * W2_BYTES + 2 * UNITS * H_BYTES + 512;
     static_assert(SMEM <= kFfnSmemMax, "shared memory budget");
 };
 
@@ -65,7 +70,11 @@ struct alignas(64) FusedArgs {
 struct FusedSmem {
     uint8_t *x, *w1, *w2, *h;
     uint64_t *x_full, *x_empty, *w1_full, *w1_empty, *w2_full, *w2_empty;
-    uint64_t *d_full, *d_free, *h_ready, *h_free, *y_full, *y_empty, *drained;  // per subtile / issuer
+    // per subtile; d_full, h_free and y_full one for even and one for odd
+    // chunks (tiles): a group may come to a chunk while another still waits
+    // for the one before, and a parity tells only two phases apart
+    uint64_t *d_full, *d_free, *h_ready, *h_free, *y_full, *y_empty, *out_ready, *out_free;
+    uint64_t* drained;  // per issuer
     uint32_t* tmem;
     int* abort;
 };
@@ -155,7 +164,7 @@ __device__ void fused_issue_d(const FusedArgs& a, const FusedSmem& S, uint32_t t
                     const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
                     umma_f16(tmem + 256 + sub * 128, sdesc_k_sw128(sx + off), sdesc_k_sw128(sw + off), idesc, ks > 0 ? 1u : 0u);
                 }
-                umma_commit(&S.d_full[sub]);
+                umma_commit(&S.d_full[sub * 2 + (c & 1)]);
                 if (j + 1 == a.chunks) umma_commit(&S.x_empty[xs]);
             }
             umma_commit(&S.w1_empty[s]);
@@ -179,14 +188,14 @@ __device__ void fused_issue_y(const FusedArgs& a, const FusedSmem& S, uint32_t t
                 if (!wait(&S.h_ready[sub], c)) return;
                 if (j == 0 && k > 0 && !wait(&S.y_empty[sub], k - 1)) return;
                 tc_fence_after();
-                const uint32_t sh = smem_u32(S.h + sub * C::H_BYTES);
+                const uint32_t sh = smem_u32(S.h + sub * C::UNITS * C::H_BYTES);
                 const uint32_t sw = smem_u32(S.w2 + s * C::W2_BYTES);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
                     umma_f16(tmem + sub * 128, sdesc_k_sw128(sh + ks * 32), sdesc_k_sw128(sw + ks * 32), idesc,
                              (j > 0 || ks > 0) ? 1u : 0u);
-                umma_commit(&S.h_free[sub]);
-                if (j + 1 == a.chunks) umma_commit(&S.y_full[sub]);
+                umma_commit(&S.h_free[sub * 2 + (c & 1)]);
+                if (j + 1 == a.chunks) umma_commit(&S.y_full[sub * 2 + (k & 1)]);
             }
             umma_commit(&S.w2_empty[s]);
         }
@@ -197,85 +206,98 @@ template <int KC>
 __device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
     using C = FusedCfg<KC>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int q = warp & 3, sub = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
+    const int q = warp & 3, half = ((warp - 4) >> 2) & 1;
     const int m = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t d = tmem + lanes + 256 + sub * 128, y = tmem + lanes + sub * 128;
-    uint8_t* unit = S.h + sub * C::H_BYTES;
-    const bool issuer = lane == 0 && half == 0 && q == 0;
-    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
-    bool ok = true;
-    int c = 0, k = 0;
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k) {
-        for (int j = 0; j < a.chunks; ++j, ++c) {
-            ok = ok && wait(&S.d_full[sub], c);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) continue;
-            tc_fence_after();
-            const int col = half * 32;
-            uint64_t g[16], u[16];
-            {
-                uint32_t rg[32], ru[32];
-                tmem_ld32(d + col, rg);
-                tmem_ld32(d + 64 + col, ru);
-                tmem_wait_ld_regs(rg);
-                tmem_wait_ld_regs(ru);
+    auto wait = [&](uint64_t* bar, int n) {
+        return __all_sync(0xffffffffu, wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status));
+    };
+    const int mine = (a.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    const int items = mine * a.chunks * 2;
+    for (int i = (warp - 4) / kGroupWarps; i < items; i += kGroups) {
+        const int sub = i & 1, c = i >> 1;      // subtile, its chunk count so far
+        const int k = c / a.chunks, j = c % a.chunks;  // this CTA's tile, chunk
+        const uint32_t d = tmem + lanes + 256 + sub * 128;
+        uint8_t* unit = S.h + sub * C::UNITS * C::H_BYTES;
+        if (!wait(&S.d_full[sub * 2 + (c & 1)], c >> 1)) return;
+        tc_fence_after();
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+            const int col = half * 32 + cc * 16;
+            uint32_t rg[16], ru[16];
+            tmem_ld16(d + col, rg);
+            tmem_ld16(d + 64 + col, ru);
+            tmem_wait_ld_regs(rg);
+            tmem_wait_ld_regs(ru);
+            if (cc == 1) {
                 tc_fence_before();
                 warp_arrive(&S.d_free[sub]);
-                to_pairs(rg, g);
-                to_pairs(ru, u);
             }
+            float g[16], u[16];
+            to_floats(rg, g);
+            to_floats(ru, u);
             add_bias(a.b_gate, j * 64 + col, a.hidden, g);
             add_bias(a.b_up, j * 64 + col, a.hidden, u);
             gate_chunk(a.act, g, u);
-            // the product of the chunk before has read the unit
-            if (c > 0) ok = wait(&S.h_free[sub], c - 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) continue;
+            if (cc == 0) {
+                // the product of the chunk before, and the store of the tile
+                // before, have read the unit
+                if (c > 0 && !wait(&S.h_free[sub * 2 + ((c - 1) & 1)], (c - 1) >> 1)) return;
+                if (j == 0 && k > 0 && !wait(&S.out_free[sub], k - 1)) return;
+            }
             put_unit(unit, m, col / 8, g, a.bf16);
-            fence_proxy_async();
-            warp_arrive(&S.h_ready[sub]);
         }
-        // the subtile's rows: through the h unit, 64 columns at a time
-        ok = ok && wait(&S.y_full[sub], k);
-        ok = __all_sync(0xffffffffu, ok);
+        fence_proxy_async();
+        warp_arrive(&S.h_ready[sub]);
+        if (j + 1 < a.chunks) continue;
+        // the subtile's last chunk: its rows out, 64 columns a unit, the last in h's
+        if (!wait(&S.y_full[sub * 2 + (k & 1)], k >> 1)) return;
         tc_fence_after();
+        const uint32_t y = tmem + lanes + sub * 128;
 #pragma unroll
-        for (int u0 = 0; u0 < C::CP; u0 += 64) {
-            if (u0 > 0) {
-                if (issuer) bulk_wait_read();
-                named_bar(1 + sub, 32 * kGroupWarps);
-            }
-            if (ok) {
+        for (int u0 = half * 32; u0 < C::CP; u0 += 64)
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    const int col = half * 32 + cc * 16;
-                    uint32_t r[16];
-                    tmem_ld16(y + u0 + col, r);
-                    tmem_wait_ld_regs(r);
-                    if (u0 + 64 == C::CP && cc == 1) {
-                        tc_fence_before();
-                        warp_arrive(&S.y_empty[sub]);
-                    }
-                    uint64_t v[8];
-                    to_pairs(r, v);
-                    add_bias(a.b_down, u0 + col, a.c, v);
-                    put_unit(unit, m, col / 8, v, a.bf16);
+            for (int cc = 0; cc < 32; cc += 16) {
+                uint32_t r[16];
+                tmem_ld16(y + u0 + cc, r);
+                tmem_wait_ld_regs(r);
+                if (u0 + 64 >= C::CP && cc == 16) {
+                    tc_fence_before();
+                    warp_arrive(&S.y_empty[sub]);
                 }
-                fence_proxy_async();
+                float v[16];
+                to_floats(r, v);
+                add_bias(a.b_down, u0 + cc, a.c, v);
+                put_unit(unit + (C::UNITS - 1 - u0 / 64) * C::H_BYTES, m, (u0 % 64 + cc) / 8, v, a.bf16);
             }
-            named_bar(1 + sub, 32 * kGroupWarps);
-            if (ok && issuer) {
-                const int row0 = tile * 256 + sub * 128;
-                if (u0 < a.c && row0 < a.rows) tma_store_2d(&a.my, smem_u32(unit), u0, row0);
-                bulk_commit();
-            }
-        }
-        // the next tile's first h waits for the store to have read the unit
-        if (issuer) bulk_wait_read();
-        named_bar(1 + sub, 32 * kGroupWarps);
+        fence_proxy_async();
+        warp_arrive(&S.out_ready[sub]);
     }
-    if (issuer) bulk_wait();
+}
+
+// Stores finished subtiles.
+template <int KC>
+__device__ void fused_store(const FusedArgs& a, const FusedSmem& S) {
+    using C = FusedCfg<KC>;
+    int k = 0;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            if (!wait_or_abort(&S.out_ready[sub], static_cast<uint32_t>(k) & 1, S.abort, a.status)) {
+                bulk_wait();
+                return;
+            }
+            const int row0 = tile * 256 + sub * 128;
+            if (row0 < a.rows)
+#pragma unroll
+                for (int u = 0; u < C::UNITS; ++u)
+                    if (u * 64 < a.c)
+                        tma_store_2d(&a.my, smem_u32(S.h + (sub * C::UNITS + C::UNITS - 1 - u) * C::H_BYTES), u * 64, row0);
+            bulk_commit();
+            bulk_wait_read();
+            mbar_arrive(&S.out_free[sub]);
+        }
+    bulk_wait();
 }
 
 template <int KC>
@@ -291,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     S.w2 = p;
     p += C::W2R * C::W2_BYTES;
     S.h = p;
-    p += 2 * C::H_BYTES;
+    p += 2 * C::UNITS * C::H_BYTES;
     S.x_full = reinterpret_cast<uint64_t*>(p);
     S.x_empty = S.x_full + C::XR;
     S.w1_full = S.x_empty + C::XR;
@@ -299,26 +321,32 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     S.w2_full = S.w1_empty + C::W1R;
     S.w2_empty = S.w2_full + C::W2R;
     S.d_full = S.w2_empty + C::W2R;
-    S.d_free = S.d_full + 2;
+    S.h_free = S.d_full + 4;
+    S.y_full = S.h_free + 4;
+    S.d_free = S.y_full + 4;
     S.h_ready = S.d_free + 2;
-    S.h_free = S.h_ready + 2;
-    S.y_full = S.h_free + 2;
-    S.y_empty = S.y_full + 2;
-    S.drained = S.y_empty + 2;
+    S.y_empty = S.h_ready + 2;
+    S.out_ready = S.y_empty + 2;
+    S.out_free = S.out_ready + 2;
+    S.drained = S.out_free + 2;
     S.tmem = reinterpret_cast<uint32_t*>(S.drained + 2);
     S.abort = reinterpret_cast<int*>(S.tmem + 1);
-    static_assert((2 * (C::XR + C::W1R + C::W2R) + 14) * 8 + 8 <= 512, "barriers fit");
+    static_assert((2 * (C::XR + C::W1R + C::W2R) + 24) * 8 + 8 <= 512, "barriers fit");
 
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2 * (C::XR + C::W1R + C::W2R); ++s) mbar_init(&S.x_full[s], 1);
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < 4; ++s) {
             mbar_init(&S.d_full[s], 1);
-            mbar_init(&S.d_free[s], kGroupWarps);
-            mbar_init(&S.h_ready[s], kGroupWarps);
             mbar_init(&S.h_free[s], 1);
             mbar_init(&S.y_full[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&S.d_free[s], kGroupWarps);
+            mbar_init(&S.h_ready[s], kGroupWarps);
             mbar_init(&S.y_empty[s], kGroupWarps);
+            mbar_init(&S.out_ready[s], kGroupWarps);
+            mbar_init(&S.out_free[s], 1);
             mbar_init(&S.drained[s], 1);
         }
         *S.abort = 0;
@@ -344,7 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
                 fused_issue_y<KC>(a, S, tmem);
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else if (warp == 3) {
+        if ((threadIdx.x & 31) == 0) fused_store<KC>(a, S);
+        __syncwarp();
+    } else {
         fused_epilogue<KC>(a, S, tmem);
     }
     tc_fence_before();

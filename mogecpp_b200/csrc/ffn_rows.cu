@@ -101,13 +101,12 @@ __global__ void __launch_bounds__(32 * kWarps) rows_hidden_kernel(const void* x,
     const float bg = w.b_gate ? __ldg(w.b_gate + j) : 0.f, bu = w.b_up ? __ldg(w.b_up + j) : 0.f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-        uint64_t a[1] = {both(warp_total(g[r]) + bg)};
-        const uint64_t b[1] = {both(warp_total(u[r]) + bu)};
+        const float tg = warp_total(g[r]) + bg, tu = warp_total(u[r]) + bu;
         if (r < n && lane == r) {
+            float a[2] = {tg, 0.f};
+            const float b[2] = {tu, 0.f};
             gate_chunk(act, a, b);
-            float v, same;
-            unpack2(a[0], v, same);
-            h[static_cast<int64_t>(r) * hidden + j] = v;
+            h[static_cast<int64_t>(r) * hidden + j] = a[0];
         }
     }
 }
