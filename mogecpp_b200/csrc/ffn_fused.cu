@@ -10,15 +10,26 @@
 //   Y += h Wd[:, chunk]^T           (TMEM, 128 rows x c columns, K = 64)
 // The weights stream through shared memory once per 256 rows (they stay in
 // L2).  The epilogue is the long pole (a gated activation an element, bound by
-// the special-function unit), so that it is kept from waiting: three groups
-// of warps take the (chunk, subtile) items in turn, each takes its D into
-// registers and releases it before it is done computing, and the next D is
-// there when a group comes back.  The two products have an issuing warp each,
-// so that neither waits for the other's operands, and a third warp stores.
+// the special-function unit and its own hand-overs), so that its warps take D
+// into registers and release it before they are done computing, and the next
+// chunk's D is there when they come back.  The two products have an issuing
+// warp each, so that neither waits for the other's operands.
+//
+// Up to 64 channels three groups of 8 warps take the (chunk, subtile) items in
+// turn, and a warp of its own stores; at 128, where the products take longer
+// and the registers of a third group would cost more than it brings (177 us
+// against 170 at 402,131 x 128 -> 512, bf16), each subtile has a group.
 //
 // TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 and 2
-// MMA issuers (D, Y), 3 TMEM allocation and stores, 4-27 epilogue (8 per
-// group: lane quarter x half of the chunk).  Every wait is bounded, as in ffn_gemm.cuh.
+// MMA issuers (D, Y), 3 TMEM allocation (and stores), 4 on epilogue (8 per
+// group: lane quarter x half of the chunk).  Every wait is bounded, as in
+// ffn_gemm.cuh.
+//
+// Measured: 402,131 x 128 -> 512 bf16 170 us (0.93 PFLOP/s; two kernels with
+// h in memory: 291 us); without the activations the products and copies alone
+// take 120 us, bound by shared-memory operand reads of 128-column products
+// and the weights' way from L2 (24 KB per item and SM).  101,117 x 64 -> 256
+// fp16 38 us (two kernels: 67 us).
 #include "ffn_fused.h"
 
 #include "common.cuh"
@@ -34,25 +45,23 @@
 namespace msc {
 namespace {
 
-constexpr int kGroups = 3;
 constexpr int kGroupWarps = 8;
-constexpr int kThreads = 32 * (4 + kGroups * kGroupWarps);
 
 // KC: 64-channel blocks of a row (c padded with zeros by the copies).
 template <int KC>
 struct FusedCfg {
+    static constexpr int GROUPS = KC == 1 ? 3 : 2;  // epilogue groups
+    static constexpr int THREADS = 32 * (4 + GROUPS * kGroupWarps);
     static constexpr int XR = KC == 1 ? 4 : 2;   // x subtile slots
-    static constexpr int W1R = KC == 1 ? 4 : 2;  // gate and up weight stages
+    static constexpr int W1R = KC == 1 ? 4 : 3;  // gate and up weight stages
     static constexpr int W2R = KC == 1 ? 4 : 2;  // down weight stages
     static constexpr int X_BYTES = KC * 128 * 128;
     static constexpr int W1_BYTES = KC * 128 * 128;  // per 64-channel block: 64 gate rows, then 64 up rows
     static constexpr int W2_BYTES = KC * 64 * 128;   // c rows of 64 hidden units
     static constexpr int H_BYTES = 128 * 128;
     static constexpr int CP = KC * 64;  // padded channels
-    // a subtile's h unit, which also takes the last 64 columns of its y on
-    // their way out, and a unit for each 64 columns before
-    static constexpr int UNITS = KC;
-    static constexpr int SMEM = 1024 + XR * X_BYTES + W1R * W1_BYTES + W2R * W2_BYTES + 2 * UNITS * H_BYTES + 512;
+    // (a subtile's h unit also takes its y out, 64 columns at a time)
+    static constexpr int SMEM = 1024 + XR * X_BYTES + W1R * W1_BYTES + W2R * W2_BYTES + 2 * H_BYTES + 512;
     static_assert(SMEM <= kFfnSmemMax, "shared memory budget");
 };
 
@@ -90,7 +99,7 @@ __device__ void fused_producer(const FusedArgs& a, const FusedSmem& S) {
     // waits until `slot` of a ring is free for its i-th use
     auto free_slot = [&](uint64_t* empty, int i, int ring) {
         return i < ring ||
-               wait_or_abort(&empty[i % ring], static_cast<uint32_t>(i / ring - 1) & 1, S.abort, a.status);
+               wait_briefly(&empty[i % ring], static_cast<uint32_t>(i / ring - 1) & 1, S.abort, a.status);
     };
     auto load_w1 = [&](int j) {
         if (!free_slot(S.w1_empty, i1, C::W1R)) return false;
@@ -146,7 +155,7 @@ __device__ void fused_issue_d(const FusedArgs& a, const FusedSmem& S, uint32_t t
     using C = FusedCfg<KC>;
     const uint32_t idesc = idesc_f16(128, 128, a.bf16 ? 1u : 0u);
     int ix = 0, c = 0;  // x slots, chunks so far
-    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    auto wait = [&](uint64_t* bar, int n) { return wait_briefly(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ix += 2) {
         for (int j = 0; j < a.chunks; ++j, ++c) {
             const int s = c % C::W1R;
@@ -178,7 +187,7 @@ __device__ void fused_issue_y(const FusedArgs& a, const FusedSmem& S, uint32_t t
     using C = FusedCfg<KC>;
     const uint32_t idesc = idesc_f16(128, C::CP, a.bf16 ? 1u : 0u);
     int c = 0, k = 0;  // chunks, tiles so far
-    auto wait = [&](uint64_t* bar, int n) { return wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    auto wait = [&](uint64_t* bar, int n) { return wait_briefly(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k) {
         for (int j = 0; j < a.chunks; ++j, ++c) {
             const int s = c % C::W2R;
@@ -188,7 +197,7 @@ __device__ void fused_issue_y(const FusedArgs& a, const FusedSmem& S, uint32_t t
                 if (!wait(&S.h_ready[sub], c)) return;
                 if (j == 0 && k > 0 && !wait(&S.y_empty[sub], k - 1)) return;
                 tc_fence_after();
-                const uint32_t sh = smem_u32(S.h + sub * C::UNITS * C::H_BYTES);
+                const uint32_t sh = smem_u32(S.h + sub * C::H_BYTES);
                 const uint32_t sw = smem_u32(S.w2 + s * C::W2_BYTES);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
@@ -202,6 +211,7 @@ __device__ void fused_issue_y(const FusedArgs& a, const FusedSmem& S, uint32_t t
     }
 }
 
+// The epilogue up to 64 channels: three groups in turn.
 template <int KC>
 __device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
     using C = FusedCfg<KC>;
@@ -210,32 +220,35 @@ __device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t 
     const int m = q * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     auto wait = [&](uint64_t* bar, int n) {
-        return __all_sync(0xffffffffu, wait_or_abort(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status));
+        return __all_sync(0xffffffffu, wait_briefly(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status));
     };
     const int mine = (a.tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
     const int items = mine * a.chunks * 2;
-    for (int i = (warp - 4) / kGroupWarps; i < items; i += kGroups) {
+    for (int i = (warp - 4) / kGroupWarps; i < items; i += C::GROUPS) {
         const int sub = i & 1, c = i >> 1;      // subtile, its chunk count so far
         const int k = c / a.chunks, j = c % a.chunks;  // this CTA's tile, chunk
         const uint32_t d = tmem + lanes + 256 + sub * 128;
-        uint8_t* unit = S.h + sub * C::UNITS * C::H_BYTES;
+        uint8_t* unit = S.h + sub * C::H_BYTES;
         if (!wait(&S.d_full[sub * 2 + (c & 1)], c >> 1)) return;
         tc_fence_after();
+        constexpr int N = 16;
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-            const int col = half * 32 + cc * 16;
-            uint32_t rg[16], ru[16];
-            tmem_ld16(d + col, rg);
-            tmem_ld16(d + 64 + col, ru);
-            tmem_wait_ld_regs(rg);
-            tmem_wait_ld_regs(ru);
-            if (cc == 1) {
-                tc_fence_before();
-                warp_arrive(&S.d_free[sub]);
+        for (int cc = 0; cc < 32; cc += N) {
+            const int col = half * 32 + cc;
+            float g[N], u[N];
+            {
+                uint32_t rg[N], ru[N];
+                tmem_ld<N>(d + col, rg);
+                tmem_ld<N>(d + 64 + col, ru);
+                tmem_wait_ld_regs(rg);
+                tmem_wait_ld_regs(ru);
+                if (cc + N == 32) {
+                    tc_fence_before();
+                    warp_arrive(&S.d_free[sub]);
+                }
+                to_floats(rg, g);
+                to_floats(ru, u);
             }
-            float g[16], u[16];
-            to_floats(rg, g);
-            to_floats(ru, u);
             add_bias(a.b_gate, j * 64 + col, a.hidden, g);
             add_bias(a.b_up, j * 64 + col, a.hidden, u);
             gate_chunk(a.act, g, u);
@@ -243,65 +256,152 @@ __device__ void fused_epilogue(const FusedArgs& a, const FusedSmem& S, uint32_t 
                 // the product of the chunk before, and the store of the tile
                 // before, have read the unit
                 if (c > 0 && !wait(&S.h_free[sub * 2 + ((c - 1) & 1)], (c - 1) >> 1)) return;
-                if (j == 0 && k > 0 && !wait(&S.out_free[sub], k - 1)) return;
+                if (j == 0 && k > 0 && !wait(&S.out_free[sub], k * KC - 1)) return;
             }
             put_unit(unit, m, col / 8, g, a.bf16);
         }
         fence_proxy_async();
         warp_arrive(&S.h_ready[sub]);
         if (j + 1 < a.chunks) continue;
-        // the subtile's last chunk: its rows out, 64 columns a unit, the last in h's
+        // the subtile's last chunk: its rows out through the unit, 64 columns at a time
         if (!wait(&S.y_full[sub * 2 + (k & 1)], k >> 1)) return;
         tc_fence_after();
         const uint32_t y = tmem + lanes + sub * 128;
 #pragma unroll
-        for (int u0 = half * 32; u0 < C::CP; u0 += 64)
+        for (int u0 = 0; u0 < C::CP; u0 += 64) {
+            if (u0 > 0 && !wait(&S.out_free[sub], k * KC + u0 / 64 - 1)) return;
 #pragma unroll
             for (int cc = 0; cc < 32; cc += 16) {
+                const int col = half * 32 + cc;
                 uint32_t r[16];
-                tmem_ld16(y + u0 + cc, r);
+                tmem_ld16(y + u0 + col, r);
                 tmem_wait_ld_regs(r);
-                if (u0 + 64 >= C::CP && cc == 16) {
+                if (u0 + 64 == C::CP && cc == 16) {
                     tc_fence_before();
                     warp_arrive(&S.y_empty[sub]);
                 }
                 float v[16];
                 to_floats(r, v);
-                add_bias(a.b_down, u0 + cc, a.c, v);
-                put_unit(unit + (C::UNITS - 1 - u0 / 64) * C::H_BYTES, m, (u0 % 64 + cc) / 8, v, a.bf16);
+                add_bias(a.b_down, u0 + col, a.c, v);
+                put_unit(unit, m, col / 8, v, a.bf16);
             }
-        fence_proxy_async();
-        warp_arrive(&S.out_ready[sub]);
+            fence_proxy_async();
+            warp_arrive(&S.out_ready[sub]);
+        }
     }
 }
 
-// Stores finished subtiles.
+// The epilogue at 128 channels: a group for each subtile, which also stores
+// its rows.
 template <int KC>
-__device__ void fused_store(const FusedArgs& a, const FusedSmem& S) {
+__device__ void fused_epilogue_pair(const FusedArgs& a, const FusedSmem& S, uint32_t tmem) {
     using C = FusedCfg<KC>;
-    int k = 0;
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k)
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int q = warp & 3, sub = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
+    const int m = q * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t d = tmem + lanes + 256 + sub * 128, y = tmem + lanes + sub * 128;
+    uint8_t* unit = S.h + sub * C::H_BYTES;
+    const bool issuer = lane == 0 && half == 0 && q == 0;
+    auto wait = [&](uint64_t* bar, int n) { return wait_briefly(bar, static_cast<uint32_t>(n) & 1, S.abort, a.status); };
+    bool ok = true;
+    int c = 0, k = 0;
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++k) {
+        for (int j = 0; j < a.chunks; ++j, ++c) {
+            ok = ok && wait(&S.d_full[sub * 2 + (c & 1)], c >> 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) continue;
+            tc_fence_after();
+            const int col = half * 32;
+            float g[32], u[32];
+            {
+                uint32_t rg[32], ru[32];
+                tmem_ld32(d + col, rg);
+                tmem_ld32(d + 64 + col, ru);
+                tmem_wait_ld_regs(rg);
+                tmem_wait_ld_regs(ru);
+                tc_fence_before();
+                warp_arrive(&S.d_free[sub]);
+                to_floats(rg, g);
+                to_floats(ru, u);
+            }
+            add_bias(a.b_gate, j * 64 + col, a.hidden, g);
+            add_bias(a.b_up, j * 64 + col, a.hidden, u);
+            gate_chunk(a.act, g, u);
+            // the product of the chunk before has read the unit
+            if (c > 0) ok = wait(&S.h_free[sub * 2 + ((c - 1) & 1)], (c - 1) >> 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) continue;
+            put_unit(unit, m, col / 8, g, a.bf16);
+            fence_proxy_async();
+            warp_arrive(&S.h_ready[sub]);
+        }
+        // the subtile's rows out through the unit, 64 columns at a time
+        ok = ok && wait(&S.y_full[sub * 2 + (k & 1)], k >> 1);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            if (!wait_or_abort(&S.out_ready[sub], static_cast<uint32_t>(k) & 1, S.abort, a.status)) {
+        for (int u0 = 0; u0 < C::CP; u0 += 64) {
+            if (u0 > 0) {
+                if (issuer) bulk_wait_read();
+                named_bar(1 + sub, 32 * kGroupWarps);
+            }
+            if (ok) {
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    const int col = half * 32 + cc * 16;
+                    uint32_t r[16];
+                    tmem_ld16(y + u0 + col, r);
+                    tmem_wait_ld_regs(r);
+                    if (u0 + 64 == C::CP && cc == 1) {
+                        tc_fence_before();
+                        warp_arrive(&S.y_empty[sub]);
+                    }
+                    float v[16];
+                    to_floats(r, v);
+                    add_bias(a.b_down, u0 + col, a.c, v);
+                    put_unit(unit, m, col / 8, v, a.bf16);
+                }
+                fence_proxy_async();
+            }
+            named_bar(1 + sub, 32 * kGroupWarps);
+            if (ok && issuer) {
+                const int row0 = tile * 256 + sub * 128;
+                if (u0 < a.c && row0 < a.rows) tma_store_2d(&a.my, smem_u32(unit), u0, row0);
+                bulk_commit();
+            }
+        }
+        // the next tile's first h waits for the store to have read the unit
+        if (issuer) bulk_wait_read();
+        named_bar(1 + sub, 32 * kGroupWarps);
+    }
+    if (issuer) bulk_wait();
+}
+
+// Stores a subtile's finished rows (one thread each).
+template <int KC>
+__device__ void fused_store(const FusedArgs& a, const FusedSmem& S, int sub) {
+    using C = FusedCfg<KC>;
+    int i = 0;  // units stored so far
+    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+        const int row0 = tile * 256 + sub * 128;
+#pragma unroll
+        for (int u = 0; u < KC; ++u, ++i) {
+            if (!wait_briefly(&S.out_ready[sub], static_cast<uint32_t>(i) & 1, S.abort, a.status)) {
                 bulk_wait();
                 return;
             }
-            const int row0 = tile * 256 + sub * 128;
-            if (row0 < a.rows)
-#pragma unroll
-                for (int u = 0; u < C::UNITS; ++u)
-                    if (u * 64 < a.c)
-                        tma_store_2d(&a.my, smem_u32(S.h + (sub * C::UNITS + C::UNITS - 1 - u) * C::H_BYTES), u * 64, row0);
+            if (row0 < a.rows && u * 64 < a.c) tma_store_2d(&a.my, smem_u32(S.h + sub * C::H_BYTES), u * 64, row0);
             bulk_commit();
             bulk_wait_read();
             mbar_arrive(&S.out_free[sub]);
         }
+    }
     bulk_wait();
 }
 
 template <int KC>
-__global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_constant__ FusedArgs a) {
+__global__ void __launch_bounds__(FusedCfg<KC>::THREADS, 1) ffn_fused_kernel(const __grid_constant__ FusedArgs a) {
     using C = FusedCfg<KC>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* p = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -313,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
     S.w2 = p;
     p += C::W2R * C::W2_BYTES;
     S.h = p;
-    p += 2 * C::UNITS * C::H_BYTES;
+    p += 2 * C::H_BYTES;
     S.x_full = reinterpret_cast<uint64_t*>(p);
     S.x_empty = S.x_full + C::XR;
     S.w1_full = S.x_empty + C::XR;
@@ -373,10 +473,13 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_fused_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp == 3) {
-        if ((threadIdx.x & 31) == 0) fused_store<KC>(a, S);
+        if (KC == 1 && (threadIdx.x & 31) < 2) fused_store<KC>(a, S, threadIdx.x & 31);
         __syncwarp();
     } else {
-        fused_epilogue<KC>(a, S, tmem);
+        if constexpr (KC == 1)
+            fused_epilogue<KC>(a, S, tmem);
+        else
+            fused_epilogue_pair<KC>(a, S, tmem);
     }
     tc_fence_before();
     __syncthreads();
@@ -417,7 +520,7 @@ cudaError_t launch_t(const FusedArgs& a, cudaStream_t st) {
         }
         sms = num_sms[dev];
     }
-    ffn_fused_kernel<KC><<<std::min(a.tiles, sms), kThreads, C::SMEM, st>>>(a);
+    ffn_fused_kernel<KC><<<std::min(a.tiles, sms), C::THREADS, C::SMEM, st>>>(a);
     return cudaGetLastError();
 }
 

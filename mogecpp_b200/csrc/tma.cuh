@@ -61,6 +61,37 @@ __device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t smem_addr, uint32_t 
     return d;
 }
 
+// wait_or_abort without a suspend hint, for the fused feed-forward block: its
+// roles hand over every few hundred cycles, and a suspended thread comes back
+// later (3 % of the block's time; the longer products of ffn_gemm.cuh lose
+// 5 % to the polling instead).
+__device__ __forceinline__ bool wait_briefly(uint64_t* bar, uint32_t parity, int* abort_flag, uint32_t* status) {
+    auto done = [&]() {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        return ok != 0;
+    };
+    if (done()) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t it = 0;; ++it) {
+        if (done()) return true;
+        if ((it & 255u) == 255u) {
+            if (*reinterpret_cast<volatile int*>(abort_flag)) return false;
+            if (global_timer_ns() - t0 > kWaitBudgetNs) {
+                atomicExch(abort_flag, 1);
+                set_status(status, MSC_DEV_TIMEOUT);
+                return false;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------- CTA pairs
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
