@@ -179,20 +179,55 @@ void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht, int cg) {
     a.ksplit = a.ksteps[0] + a.ksteps[1];
 }
 
+// Column sums of a 16-bit [n][c] matrix over a run of rows per block, fp32.
+constexpr int kColsumRows = 256;
+__global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, int lanes, float* part) {
+    // `lanes` threads (8, 16 or 32) x 8 columns a row, 256 / lanes rows at once
+    __shared__ float red[256][9];
+    const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, ry = 256 / lanes;
+    const int col = (blockIdx.y * lanes + tx) * 8;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kColsumRows;
+    const int64_t r1 = min(r0 + kColsumRows, n);
+    float s[8] = {};
+    if (col < c) {
+#pragma unroll 4
+        for (int64_t r = r0 + ty; r < r1; r += ry) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(y) + r * c + col);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 t = bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
+                                      : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                s[2 * e] += t.x, s[2 * e + 1] += t.y;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[threadIdx.x][e] = s[e];
+    __syncthreads();
+    for (int o = threadIdx.x; o < lanes * 8; o += 256) {
+        const int t = o >> 3, e = o & 7;
+        const int cc = (blockIdx.y * lanes + t) * 8 + e;
+        if (cc >= c) continue;
+        float q = 0.f;
+        for (int w = 0; w < ry; ++w) q += red[w * lanes + t][e];
+        part[static_cast<int64_t>(blockIdx.x) * c + cc] = q;
+    }
+}
+
 // out[i] = sum over the splits of part[s][i] (+ bias of column i % cols), in
 // split order; four elements a thread.
-struct SplitSumArgs {
+struct SplitSum {
     const float* part;
     int64_t stride;      // floats per split
     int splits;
     void* out[3];
-    int64_t begin[4];    // first element of each output, and the end
+    int64_t begin[4];    // first element of each output, and the end (0: nothing to do)
     const float* bias;
     int cols;
-    int bf16;
 };
-__global__ void __launch_bounds__(256) split_sum_kernel(const SplitSumArgs a) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+__device__ void split_sum(const SplitSum& a, int64_t block, int bf16) {
+    const int64_t i = (block * 256 + threadIdx.x) * 4;
     if (i >= a.begin[3]) return;
     float4 s = *reinterpret_cast<const float4*>(a.part + i);
     for (int k = 1; k < a.splits; ++k) {
@@ -205,80 +240,69 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const SplitSumArgs a) {
     }
     const int p = i >= a.begin[2] ? 2 : (i >= a.begin[1] ? 1 : 0);
     uint2 w;
-    if (a.bf16) {
+    if (bf16) {
         const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
         w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     } else {
         const __half2 lo = __floats2half2_rn(s.x, s.y), hi = __floats2half2_rn(s.z, s.w);
         w = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out[p]) + (i - a.begin[p])) = w;
+    uint16_t* out = static_cast<uint16_t*>(p == 2 ? a.out[2] : (p == 1 ? a.out[1] : a.out[0]));
+    *reinterpret_cast<uint2*>(out + (i - (p == 2 ? a.begin[2] : (p == 1 ? a.begin[1] : a.begin[0])))) = w;
 }
 
-cudaError_t launch_split_sum(const SplitSumArgs& a, cudaStream_t st) {
-    split_sum_kernel<<<static_cast<unsigned>(cdiv(a.begin[3], 1024)), 256, 0, st>>>(a);
-    return cudaGetLastError();
-}
-
-// Column sums of a 16-bit [n][c] matrix over a run of rows per block, fp32.
-constexpr int kColsumRows = 256;
-__global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, float* part) {
-    // 32 threads x 8 columns, 8 rows in flight
-    __shared__ float red[8][32][9];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int col = (blockIdx.y * 32 + tx) * 8;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kColsumRows;
-    const int64_t r1 = min(r0 + kColsumRows, n);
-    float s[8] = {};
-    if (col < c)
-        for (int64_t r = r0 + ty; r < r1; r += 8) {
-            const uint4 w4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(y) + r * c + col);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 t = bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
-                                      : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                s[2 * e] += t.x, s[2 * e + 1] += t.y;
-            }
-        }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) red[ty][tx][e] = s[e];
-    __syncthreads();
-    if (ty == 0 && col < c) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float q = 0.f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) q += red[w][tx][e];
-            part[static_cast<int64_t>(blockIdx.x) * c + col + e] = q;
-        }
-    }
-}
-
-// Totals over the units of part [units][cols] in double and in a fixed order;
-// the first n0 columns go to out0, the others to out1 (either may be NULL).
-__global__ void __launch_bounds__(1024) column_total_kernel(const float* part, int64_t units, int cols, int n0,
-                                                            float* out0, float* out1) {
-    __shared__ double red[32][33];
-    const int col = blockIdx.x * 32 + threadIdx.x;
+// Totals over the units of part [units][cols] in double and in a fixed order,
+// 8 columns a block; the first n0 columns go to out[0], the others to out[1]
+// (either may be NULL).
+struct ColumnTotal {
+    const float* part;
+    int64_t units;
+    int cols, n0;  // cols 0: nothing to do
+    float* out[2];
+};
+__device__ void column_total(const ColumnTotal& a, int block) {
+    __shared__ double red[32][9];
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int col = block * 8 + tx;
     double s = 0.0;
-    if (col < cols)
-        for (int64_t u = threadIdx.y; u < units; u += 32) s += part[u * cols + col];
-    red[threadIdx.y][threadIdx.x] = s;
+    if (col < a.cols) {
+#pragma unroll 8
+        for (int64_t u = ty; u < a.units; u += 32) s += a.part[u * a.cols + col];
+    }
+    red[ty][tx] = s;
     __syncthreads();
     for (int o = 16; o >= 1; o >>= 1) {
-        if (threadIdx.y < o) red[threadIdx.y][threadIdx.x] += red[threadIdx.y + o][threadIdx.x];
+        if (ty < o) red[ty][tx] += red[ty + o][tx];
         __syncthreads();
     }
-    if (threadIdx.y == 0 && col < cols) {
-        float* o = col < n0 ? out0 : out1;
-        if (o) o[col < n0 ? col : col - n0] = static_cast<float>(red[0][threadIdx.x]);
+    if (ty == 0 && col < a.cols) {
+        float* o = col < a.n0 ? a.out[0] : a.out[1];
+        if (o) o[col < a.n0 ? col : col - a.n0] = static_cast<float>(red[0][tx]);
     }
 }
 
-cudaError_t launch_column_total(const float* part, int64_t units, int cols, int n0, float* out0, float* out1,
-                                cudaStream_t st) {
-    column_total_kernel<<<static_cast<unsigned>(cdiv(cols, 32)), dim3(32, 32), 0, st>>>(part, units, cols, n0, out0, out1);
+// What is left of a pass after its products, in one launch: the K splits'
+// sums and the bias gradients' column totals.
+struct FinishArgs {
+    SplitSum split[2];
+    ColumnTotal total[2];
+    int end[4];  // last block (exclusive) of split[0], split[1], total[0], total[1]
+    int bf16;
+};
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishArgs a) {
+    const int b = blockIdx.x;
+    if (b < a.end[0]) split_sum(a.split[0], b, a.bf16);
+    else if (b < a.end[1]) split_sum(a.split[1], b - a.end[0], a.bf16);
+    else if (b < a.end[2]) column_total(a.total[0], b - a.end[1]);
+    else column_total(a.total[1], b - a.end[2]);
+}
+
+cudaError_t launch_finish(FinishArgs& a, cudaStream_t st) {
+    int64_t end = 0;
+    for (int i = 0; i < 2; ++i) a.end[i] = static_cast<int>(end += cdiv(a.split[i].begin[3], 1024));
+    for (int i = 0; i < 2; ++i) a.end[2 + i] = static_cast<int>(end += cdiv(a.total[i].cols, 8));
+    if (end == 0) return cudaSuccess;
+    finish_kernel<<<static_cast<unsigned>(end), 256, 0, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -298,7 +322,7 @@ struct FwdWs {
 FwdWs fwd_ws(int64_t n, int c, int hidden) {
     FwdWs w{};
     if (use_fused(n, c)) return w;
-    if (n <= kFfnFewRows) {
+    if (ffn_few_rows(n, c, hidden)) {
         w.total = align256(static_cast<size_t>(n) * hidden * 4);
         return w;
     }
@@ -310,7 +334,7 @@ FwdWs fwd_ws(int64_t n, int c, int hidden) {
 }
 
 struct BwdWs {
-    size_t dg, du, h, bias, dbd, part, total;
+    size_t dg, du, h, bias, dbd, part_x, part_w, total;
 };
 BwdWs bwd_ws(int64_t n, int c, int hidden) {
     BwdWs w{};
@@ -320,12 +344,11 @@ BwdWs bwd_ws(int64_t n, int c, int hidden) {
     w.h = 2 * nh;
     w.bias = 3 * nh;
     w.dbd = w.bias + align256(static_cast<size_t>(cdiv(n, 128)) * 2 * hidden * 4);
-    w.part = w.dbd + align256(static_cast<size_t>(cdiv(n, kColsumRows)) * c * 4);
+    w.part_x = w.dbd + align256(static_cast<size_t>(cdiv(n, kColsumRows)) * c * 4);
     const ProjPlan px = proj_plan(n, c, static_cast<int>(2 * cdiv(hidden, 64)));
     const DwPlan pw = dw_plan(n, c, hidden);
-    size_t part = px.splits > 1 ? static_cast<size_t>(px.splits) * n * c * 4 : 0;
-    if (pw.splits > 1) part = std::max(part, static_cast<size_t>(pw.splits) * 3 * c * hidden * 4);
-    w.total = w.part + align256(part);
+    w.part_w = w.part_x + (px.splits > 1 ? align256(static_cast<size_t>(px.splits) * n * c * 4) : 0);
+    w.total = w.part_w + (pw.splits > 1 ? align256(static_cast<size_t>(pw.splits) * 3 * c * hidden * 4) : 0);
     return w;
 }
 
@@ -352,7 +375,7 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
                        cudaStream_t st) {
     if (s.n == 0) return cudaSuccess;
     if (use_fused(s.n, s.c)) return launch_ffn_fused(s, x, w, y, status, st);
-    if (s.n <= kFfnFewRows) return launch_ffn_rows(s, x, w, y, static_cast<float*>(ws), st);
+    if (ffn_few_rows(s.n, s.c, s.hidden)) return launch_ffn_rows(s, x, w, y, static_cast<float*>(ws), st);
     const bool bf = s.dtype == DT_BF16;
     const FwdWs o = fwd_ws(s.n, s.c, s.hidden);
     char* base = static_cast<char*>(ws);
@@ -390,8 +413,10 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
     MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, p.cg, st));
     if (p.splits > 1) {
         const int64_t e = s.n * s.c;
-        const SplitSumArgs r{a.partial, e, p.splits, {y, nullptr, nullptr}, {0, e, e, e}, w.b_down, s.c, bf};
-        MSC_TRY(launch_split_sum(r, st));
+        FinishArgs f{};
+        f.split[0] = SplitSum{a.partial, e, p.splits, {y, nullptr, nullptr}, {0, e, e, e}, w.b_down, s.c};
+        f.bf16 = bf;
+        MSC_TRY(launch_finish(f, st));
     }
     return cudaSuccess;
 }
@@ -416,7 +441,8 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
     void* dg = base + o.dg;
     void* du = base + o.du;
     void* h = base + o.h;
-    float* part = reinterpret_cast<float*>(base + o.part);
+    FinishArgs fin{};
+    fin.bf16 = bf;
     const int kc = static_cast<int>(cdiv(s.c, 64)), kh = static_cast<int>(cdiv(s.hidden, 64));
     const int64_t m = cdiv(s.n, 128);
     {
@@ -437,15 +463,16 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
         if (g.b_gate || g.b_up) a.bias_part = reinterpret_cast<float*>(base + o.bias);
         a.act = s.act, a.bf16 = bf, a.status = status;
         MSC_TRY(launch_gemm<FFN_HBACK>(a, ht, cg, st));
-        if (a.bias_part) MSC_TRY(launch_column_total(a.bias_part, m, 2 * s.hidden, s.hidden, g.b_gate, g.b_up, st));
+        if (a.bias_part) fin.total[0] = ColumnTotal{a.bias_part, m, 2 * s.hidden, s.hidden, {g.b_gate, g.b_up}};
     }
     if (g.b_down) {
         float* cp = reinterpret_cast<float*>(base + o.dbd);
         const int64_t units = cdiv(s.n, kColsumRows);
-        colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 256))), 256, 0, st>>>(
-            dy, s.n, s.c, bf, cp);
+        const int lanes = s.c <= 64 ? 8 : (s.c <= 128 ? 16 : 32);
+        colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 8 * lanes))), 256, 0, st>>>(
+            dy, s.n, s.c, bf, lanes, cp);
         MSC_TRY(cudaGetLastError());
-        MSC_TRY(launch_column_total(cp, units, s.c, s.c, g.b_down, nullptr, st));
+        fin.total[1] = ColumnTotal{cp, units, s.c, s.c, {g.b_down, nullptr}};
     }
     if (g.dx) {
         FfnGemmArgs a{};
@@ -460,15 +487,12 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
         a.splits = p.splits, a.ksplit = p.ksplit;
         a.bf16 = bf, a.status = status;
         if (p.splits > 1) {
-            a.partial = part;
-            a.partial_split = s.n * s.c;
+            const int64_t e = s.n * s.c;
+            a.partial = reinterpret_cast<float*>(base + o.part_x);
+            a.partial_split = e;
+            fin.split[0] = SplitSum{a.partial, e, p.splits, {g.dx, nullptr, nullptr}, {0, e, e, e}, nullptr, s.c};
         }
         MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, p.cg, st));
-        if (p.splits > 1) {
-            const int64_t e = s.n * s.c;
-            const SplitSumArgs r{part, e, p.splits, {g.dx, nullptr, nullptr}, {0, e, e, e}, nullptr, s.c, bf};
-            MSC_TRY(launch_split_sum(r, st));
-        }
     }
     if (g.w_gate) {
         FfnGemmArgs a{};
@@ -492,16 +516,13 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
         a.splits = p.splits, a.ksplit = p.ksplit;
         a.bf16 = bf, a.status = status;
         if (p.splits > 1) {
-            a.partial = part;
+            a.partial = reinterpret_cast<float*>(base + o.part_w);
             a.partial_split = 3 * ch;
+            fin.split[1] = SplitSum{a.partial, 3 * ch, p.splits, {om[0], om[1], om[2]}, {0, ch, 2 * ch, 3 * ch}, nullptr, s.c};
         }
         MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, p.cg, st));
-        if (p.splits > 1) {
-            const SplitSumArgs r{part, 3 * ch, p.splits, {om[0], om[1], om[2]}, {0, ch, 2 * ch, 3 * ch}, nullptr, s.c, bf};
-            MSC_TRY(launch_split_sum(r, st));
-        }
     }
-    return cudaSuccess;
+    return launch_finish(fin, st);
 }
 
 }  // namespace msc

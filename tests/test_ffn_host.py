@@ -13,7 +13,9 @@ from mogecpp_b200.sparse import SparseCudaExecutor
 def test_workspace_queries():
     lib = L.load()
     # the hidden values in 16 bits, then the K split's partial sums where few rows leave SMs idle
-    assert lib.msc_gated_ffn_workspace_bytes(100000, 128, 512) == 100000 * 512 * 2
+    assert lib.msc_gated_ffn_workspace_bytes(100000, 256, 512) == 100000 * 512 * 2
+    # one kernel keeps them on the SM where the channels are few and the rows many
+    assert lib.msc_gated_ffn_workspace_bytes(100000, 128, 512) == 0
     assert lib.msc_gated_ffn_workspace_bytes(1, 1024, 4096) >= 4096 * 2
     assert lib.msc_gated_ffn_workspace_bytes(0, 128, 512) >= 0
     for bad in ((-1, 128, 512), (1, 0, 512), (1, 128, 0), (1, 8200, 512), (1, 128, 65544), (1 << 40, 128, 512)):
@@ -38,9 +40,9 @@ def test_workspace_queries():
 def test_sizes_grow_with_rows():
     lib = L.load()
     for q in (lib.msc_gated_ffn_workspace_bytes, lib.msc_gated_ffn_backward_workspace_bytes):
-        assert q(2000000, 128, 512) > q(1000000, 128, 512) > q(100000, 128, 512) > 0
+        assert q(2000000, 256, 512) > q(1000000, 256, 512) > q(100000, 256, 512) > 0
         # past 32 bits
-        assert q(70000000, 128, 512) > 1 << 32
+        assert q(70000000, 256, 512) > 1 << 32
 
 
 def test_null_context_is_refused():
