@@ -512,7 +512,7 @@ typedef struct {
     msc_norm post;
     msc_norm pre;
     const float* gate; /* NULL: ones; nsamples = 0: [c]; else [nsamples][c] */
-    int nsamples;      /* a row's sample is coords[i][3] (only read with a gate per sample) */
+    int nsamples;      /* a row's sample is coords[i][3] (only read with a gate per sample); at most 32768 */
     float res_scale;
 } msc_residual_norm_desc;
 

@@ -996,7 +996,7 @@ msc::RowNormArgs rownorm_args(msc_ctx_t ctx, const msc_residual_norm_desc* d, in
     a.gate = branch ? d->gate : nullptr;
     need_aligned(a.gate, 16, "gate");
     if (a.gate) {
-        need(d->nsamples >= 0 && d->nsamples <= (1 << 20), "nsamples out of range");
+        need(d->nsamples >= 0 && d->nsamples <= msc::kRowNormMaxSamples, "nsamples out of range");
         a.nsamples = d->nsamples;
         if (d->nsamples) {
             need(coords != nullptr || n == 0, "a gate per sample needs the coordinates");
@@ -1067,7 +1067,7 @@ int msc_residual_norm(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t
 }
 
 size_t msc_residual_norm_backward_workspace_bytes(int64_t n, int c, int nsamples) {
-    if (n < 0 || c <= 0 || c > msc::kRowNormMaxC || nsamples < 0 || nsamples > (1 << 20)) return 0;
+    if (n < 0 || c <= 0 || c > msc::kRowNormMaxC || nsamples < 0 || nsamples > msc::kRowNormMaxSamples) return 0;
     return align256(msc::rownorm_backward_workspace_bytes(n, c, nsamples));
 }
 
@@ -1117,11 +1117,12 @@ int msc_gated_ffn(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const voi
         need_ctx(ctx);
         const FfnCall k = ffn_call(ffn, n, c);
         if (n == 0) return;
-        need(x && y && ws, "null pointer");
+        const size_t want = msc::ffn_workspace_bytes(n, c, ffn->hidden);
+        need(x && y && (ws || want == 0), "null pointer");
         need_aligned(x, 16, "x");
         need_aligned(y, 16, "y");
         need_aligned(ws, 256, "workspace");
-        need_ws(ws_bytes, msc::ffn_workspace_bytes(n, c, ffn->hidden));
+        need_ws(ws_bytes, want);
         ProfScope ps(ctx, "gated_ffn", S(stream));
         cuda_ok(msc::launch_ffn(k.s, x, k.w, y, ws, ctx->status, S(stream)), "gated ffn launch");
     });

@@ -180,14 +180,17 @@ void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht, int cg) {
 }
 
 // Column sums of a 16-bit [n][c] matrix over a run of rows per block, fp32.
-constexpr int kColsumRows = 256;
-__global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, int lanes, float* part) {
+// Rows of a run: few where the rows are few, so that more SMs have loads in
+// flight (1,237 x 256: 3.4 us with 64, 8.2 with 256); more runs cost their
+// totals (101,117 x 128: 13.1 + 6.5 us with 256, 10.9 + 10.0 with 64).
+int colsum_rows(int64_t n) { return n <= 16384 ? 64 : 256; }
+__global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, int lanes, int run, float* part) {
     // `lanes` threads (8, 16 or 32) x 8 columns a row, 256 / lanes rows at once
     __shared__ float red[256][9];
     const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, ry = 256 / lanes;
     const int col = (blockIdx.y * lanes + tx) * 8;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kColsumRows;
-    const int64_t r1 = min(r0 + kColsumRows, n);
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * run;
+    const int64_t r1 = min(r0 + run, n);
     float s[8] = {};
     if (col < c) {
 #pragma unroll 4
@@ -344,7 +347,7 @@ BwdWs bwd_ws(int64_t n, int c, int hidden) {
     w.h = 2 * nh;
     w.bias = 3 * nh;
     w.dbd = w.bias + align256(static_cast<size_t>(cdiv(n, 128)) * 2 * hidden * 4);
-    w.part_x = w.dbd + align256(static_cast<size_t>(cdiv(n, kColsumRows)) * c * 4);
+    w.part_x = w.dbd + align256(static_cast<size_t>(cdiv(n, colsum_rows(n))) * c * 4);
     const ProjPlan px = proj_plan(n, c, static_cast<int>(2 * cdiv(hidden, 64)));
     const DwPlan pw = dw_plan(n, c, hidden);
     w.part_w = w.part_x + (px.splits > 1 ? align256(static_cast<size_t>(px.splits) * n * c * 4) : 0);
@@ -467,10 +470,10 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
     }
     if (g.b_down) {
         float* cp = reinterpret_cast<float*>(base + o.dbd);
-        const int64_t units = cdiv(s.n, kColsumRows);
+        const int64_t units = cdiv(s.n, colsum_rows(s.n));
         const int lanes = s.c <= 64 ? 8 : (s.c <= 128 ? 16 : 32);
         colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 8 * lanes))), 256, 0, st>>>(
-            dy, s.n, s.c, bf, lanes, cp);
+            dy, s.n, s.c, bf, lanes, colsum_rows(s.n), cp);
         MSC_TRY(cudaGetLastError());
         fin.total[1] = ColumnTotal{cp, units, s.c, s.c, {g.b_down, nullptr}};
     }

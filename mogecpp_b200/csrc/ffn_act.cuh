@@ -49,6 +49,14 @@ __device__ __forceinline__ uint64_t sigmoid2(uint64_t v) {
 constexpr float kGelu0 = 1.5957691216057308f;   // 2 sqrt(2/pi)
 constexpr float kGelu1 = 0.07135481282553484f;  // 2 sqrt(2/pi) 0.044715
 
+// g held at -15, below which GELU and its derivative are under 2^-300: sigma's
+// floor times the cube in the derivative would grow again far out.  NaN stays.
+__device__ __forceinline__ uint64_t gelu_floor2(uint64_t g) {
+    float a, b;
+    unpack2(g, a, b);
+    return pack2(a < -15.0f ? -15.0f : a, b < -15.0f ? -15.0f : b);
+}
+
 // Phi(g) = (1 + erf(g / sqrt 2)) / 2 by Abramowitz and Stegun's 7.1.26
 // (|error| <= 1.5e-7 in erf): erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2), t =
 // 1 / (1 + p z), for z = |g| / sqrt 2, reflected for g > 0.  gauss is
@@ -72,6 +80,7 @@ __device__ __forceinline__ uint64_t act_value(uint64_t g) {
     if constexpr (ACT == ACT_SILU) {
         return mul2(g, sigmoid2(g));
     } else if constexpr (ACT == ACT_GELU) {
+        g = gelu_floor2(g);
         return mul2(g, sigmoid2(mul2(g, fma2(mul2(g, g), both(kGelu1), both(kGelu0)))));
     } else {
         uint64_t gauss;
@@ -88,6 +97,7 @@ __device__ __forceinline__ void act_both(uint64_t g, uint64_t& v, uint64_t& dv) 
         v = mul2(g, s);
         dv = fma2(v, fma2(s, minus, one), s);
     } else if constexpr (ACT == ACT_GELU) {
+        g = gelu_floor2(g);
         const uint64_t gg = mul2(g, g);
         const uint64_t s = sigmoid2(mul2(g, fma2(gg, both(kGelu1), both(kGelu0))));
         v = mul2(g, s);

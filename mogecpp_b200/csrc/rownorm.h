@@ -50,6 +50,7 @@ struct RowNormGrads {
 };
 
 constexpr int kRowNormMaxC = 8192;
+constexpr int kRowNormMaxSamples = 1 << 15;
 
 bool rownorm_dtypes_supported(int x_dtype, int f_dtype);
 cudaError_t launch_rownorm(const RowNormArgs& a, cudaStream_t st);

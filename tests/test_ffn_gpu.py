@@ -81,10 +81,10 @@ def check(got, want, bound, what):
 
 
 # lengths of one, below and above a tile, channels and hidden sizes that end inside a tile of 64 / 128 / 256,
-# few rows (K split) and many
+# few rows (dot products, K split), many (one kernel up to 128 channels, CTA pairs)
 SHAPES = [(1, 64, 64), (1, 1024, 2048), (3, 8, 8), (8, 128, 512), (9, 128, 520), (127, 64, 256), (128, 128, 512),
           (129, 136, 344), (300, 264, 72), (1237, 512, 1376), (5000, 72, 200), (20000, 128, 512), (20001, 64, 176),
-          (2000, 1024, 1032)]
+          (2000, 1024, 1032), (19001, 8, 8), (19201, 120, 72), (10007, 264, 520), (4097, 1024, 2056)]
 
 
 @pytest.mark.parametrize("n,c,hidden", SHAPES)
@@ -227,6 +227,46 @@ def test_large_values_stay_finite(ex):
         check(y, want, bound, act)
         g = ex.gated_ffn_backward(x, dy, ffn, act=act)
         assert all(v.isfinite().all() for v in g.values())
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_erf"])
+def test_far_out_gates(ex, act):
+    """Gates of exactly -3e5 ... 3e5 (identity weights, fp32-exact products):
+    far below zero the value and the derivative are zero (to |g| 2^-62, the
+    floor of sigma), far above g and one; a 16-bit rounding each."""
+    c = 16
+    g = torch.tensor([-3e5, -1e4, -300., -40., -8., -2., -0.5, 0., 0.5, 2., 8., 40., 300., 1e4, 3e5, 1.],
+                     device="cuda").to(torch.bfloat16)
+    x = g.repeat(40, 1).contiguous()
+    eye = torch.eye(c, device="cuda", dtype=torch.bfloat16)
+    ffn = dict(w_gate=eye, w_up=torch.zeros_like(eye), w_down=eye, b_up=torch.ones(c, device="cuda"))
+    v, dv = act64(g.double(), act)
+    y = ex.gated_ffn(x, ffn, act=act)
+    u = 2.0 ** -8
+    assert ((y.double() - v).abs() <= 2 * u * v.abs() + 1e-6).all()
+    got = ex.gated_ffn_backward(x, torch.ones_like(x), ffn, act=act)
+    assert ((got["x"].double() - dv).abs() <= 2 * u * dv.abs() + 1e-6).all()
+    ex.check()
+
+
+@pytest.mark.parametrize("n,c,hidden", [(1, 256, 1032), (6, 128, 344), (20001, 64, 176), (19500, 128, 344),
+                                        (10000, 264, 520)])
+def test_every_path_captured(ex, n, c, hidden):
+    """A first call inside a capture, replayed on new data in the same buffers:
+    the two launches of few rows, the single kernel, the CTA pairs."""
+    x, dy, ffn = make(70 + n, n, c, hidden, torch.bfloat16, True)
+    other = make(71 + n, n, c, hidden, torch.bfloat16, True)[0]
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = ex.gated_ffn(x, ffn)
+        g = ex.gated_ffn_backward(x, dy, ffn)
+    for data in (x.clone(), other):
+        x.copy_(data)
+        gr.replay()
+        assert torch.equal(y, ex.gated_ffn(data, ffn))
+        want = ex.gated_ffn_backward(data, dy, ffn)
+        assert all(torch.equal(g[k], want[k]) for k in want)
+    ex.check()
 
 
 def test_streams_and_graphs(ex):

@@ -27,7 +27,7 @@ def test_workspace_queries():
     # two row buffers and the block's own
     assert lib.msc_ffn_stack_workspace_bytes(1000, 128, 512) == (
         2 * 1000 * 128 * 2 + lib.msc_gated_ffn_workspace_bytes(1000, 128, 512))
-    for n, c, ns in ((1, 8, 0), (400000, 128, 2), (400000, 128, 127), (1000, 8192, 1 << 20)):
+    for n, c, ns in ((1, 8, 0), (400000, 128, 2), (400000, 128, 127), (1000, 8192, 1 << 15)):
         b = lib.msc_residual_norm_backward_workspace_bytes(n, c, ns)
         assert b >= (4 + max(ns, 1)) * c * 4
         # the slabs of all units stay within 64 MiB unless one alone is larger
@@ -35,6 +35,7 @@ def test_workspace_queries():
     assert lib.msc_residual_norm_backward_workspace_bytes(-1, 128, 0) == 0
     assert lib.msc_residual_norm_backward_workspace_bytes(1, 8200, 0) == 0
     assert lib.msc_residual_norm_backward_workspace_bytes(1, 128, -1) == 0
+    assert lib.msc_residual_norm_backward_workspace_bytes(1, 128, (1 << 15) + 1) == 0
 
 
 def test_sizes_grow_with_rows():
