@@ -109,20 +109,31 @@ DwPlan dw_plan(int64_t n, int c, int hidden) {
     return p;
 }
 
+// Lets a kernel of a pass start while the one before it drains (it waits for
+// it before it touches memory): 1,237 x 512 -> 1376 takes 19.1 us for 20.7.  A
+// pass's first kernel is launched without it, after all earlier work.
+cudaLaunchAttribute overlap_attribute() {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    return at;
+}
+
 template <int MODE, int HT, int CG>
-cudaError_t launch_gemm_t(const FfnGemmArgs& a, cudaStream_t st) {
+cudaError_t launch_gemm_t(const FfnGemmArgs& a, bool first, cudaStream_t st) {
     using C = FfnCfg<MODE, HT, CG>;
     auto kern = ffn_gemm_kernel<MODE, HT, CG>;
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = CG;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1] = overlap_attribute();
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
     // per device and instantiation: the shared-memory opt-in and the CTAs
     // (pairs) that run at once, set up once under a lock
     static std::mutex mu;
@@ -151,20 +162,21 @@ cudaError_t launch_gemm_t(const FfnGemmArgs& a, cudaStream_t st) {
         running = at_once[dev];
     }
     cfg.gridDim = dim3(static_cast<unsigned>(CG * std::min(a.tiles * a.splits, running)));
+    cfg.numAttrs = first ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int MODE>
-cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, int cg, cudaStream_t st) {
+cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, int cg, bool first, cudaStream_t st) {
     if constexpr (MODE == FFN_HBACK) {
-        return cg == 2 ? launch_gemm_t<MODE, 128, 2>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
+        return cg == 2 ? launch_gemm_t<MODE, 128, 2>(a, first, st) : launch_gemm_t<MODE, 64, 1>(a, first, st);
     } else if constexpr (MODE == FFN_HIDDEN) {
-        if (cg == 2) return launch_gemm_t<MODE, 128, 2>(a, st);
-        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
+        if (cg == 2) return launch_gemm_t<MODE, 128, 2>(a, first, st);
+        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, first, st) : launch_gemm_t<MODE, 64, 1>(a, first, st);
     } else {
-        if (cg == 2) return ht == 256 ? launch_gemm_t<MODE, 256, 2>(a, st) : launch_gemm_t<MODE, 128, 2>(a, st);
-        if (ht == 256) return launch_gemm_t<MODE, 256, 1>(a, st);
-        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, st) : launch_gemm_t<MODE, 64, 1>(a, st);
+        if (cg == 2) return ht == 256 ? launch_gemm_t<MODE, 256, 2>(a, first, st) : launch_gemm_t<MODE, 128, 2>(a, first, st);
+        if (ht == 256) return launch_gemm_t<MODE, 256, 1>(a, first, st);
+        return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, first, st) : launch_gemm_t<MODE, 64, 1>(a, first, st);
     }
 }
 
@@ -186,6 +198,7 @@ void one_problem(FfnGemmArgs& a, int64_t rows, int cols, int ht, int cg) {
 int colsum_rows(int64_t n) { return n <= 16384 ? 64 : 256; }
 __global__ void __launch_bounds__(256) colsum_kernel(const void* y, int64_t n, int c, int bf16, int lanes, int run, float* part) {
     // `lanes` threads (8, 16 or 32) x 8 columns a row, 256 / lanes rows at once
+    launch_dependents();
     __shared__ float red[256][9];
     const int tx = threadIdx.x & (lanes - 1), ty = threadIdx.x / lanes, ry = 256 / lanes;
     const int col = (blockIdx.y * lanes + tx) * 8;
@@ -293,6 +306,7 @@ struct FinishArgs {
     int bf16;
 };
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishArgs a) {
+    wait_dependency();
     const int b = blockIdx.x;
     if (b < a.end[0]) split_sum(a.split[0], b, a.bf16);
     else if (b < a.end[1]) split_sum(a.split[1], b - a.end[0], a.bf16);
@@ -305,8 +319,14 @@ cudaError_t launch_finish(FinishArgs& a, cudaStream_t st) {
     for (int i = 0; i < 2; ++i) a.end[i] = static_cast<int>(end += cdiv(a.split[i].begin[3], 1024));
     for (int i = 0; i < 2; ++i) a.end[2 + i] = static_cast<int>(end += cdiv(a.total[i].cols, 8));
     if (end == 0) return cudaSuccess;
-    finish_kernel<<<static_cast<unsigned>(end), 256, 0, st>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(end));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at = overlap_attribute();
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, finish_kernel, a);
 }
 
 #define MSC_TRY(expr)                        \
@@ -397,7 +417,7 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
         one_problem(a, s.n, s.hidden, ht, cg);
         a.bias0 = w.b_gate, a.bias1 = w.b_up;
         a.act = s.act, a.bf16 = bf, a.status = status;
-        MSC_TRY(launch_gemm<FFN_HIDDEN>(a, ht, cg, st));
+        MSC_TRY(launch_gemm<FFN_HIDDEN>(a, ht, cg, true, st));
     }
     FfnGemmArgs a{};
     a.ksteps[0] = static_cast<int>(cdiv(s.hidden, 64));
@@ -413,7 +433,7 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
         a.partial = reinterpret_cast<float*>(base + o.part);
         a.partial_split = s.n * s.c;
     }
-    MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, p.cg, st));
+    MSC_TRY(launch_gemm<FFN_PROJ>(a, p.ht, p.cg, false, st));
     if (p.splits > 1) {
         const int64_t e = s.n * s.c;
         FinishArgs f{};
@@ -448,6 +468,15 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
     fin.bf16 = bf;
     const int kc = static_cast<int>(cdiv(s.c, 64)), kh = static_cast<int>(cdiv(s.hidden, 64));
     const int64_t m = cdiv(s.n, 128);
+    if (g.b_down) {
+        float* cp = reinterpret_cast<float*>(base + o.dbd);
+        const int64_t units = cdiv(s.n, colsum_rows(s.n));
+        const int lanes = s.c <= 64 ? 8 : (s.c <= 128 ? 16 : 32);
+        colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 8 * lanes))), 256, 0, st>>>(
+            dy, s.n, s.c, bf, lanes, colsum_rows(s.n), cp);
+        MSC_TRY(cudaGetLastError());
+        fin.total[1] = ColumnTotal{cp, units, s.c, s.c, {g.b_down, nullptr}};
+    }
     {
         FfnGemmArgs a{};
         const int cg = cdiv(s.n, 256) * cdiv(s.hidden, 128) >= kSms / 2 ? 2 : 1;
@@ -465,17 +494,8 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
         a.bias0 = w.b_gate, a.bias1 = w.b_up;
         if (g.b_gate || g.b_up) a.bias_part = reinterpret_cast<float*>(base + o.bias);
         a.act = s.act, a.bf16 = bf, a.status = status;
-        MSC_TRY(launch_gemm<FFN_HBACK>(a, ht, cg, st));
+        MSC_TRY(launch_gemm<FFN_HBACK>(a, ht, cg, !g.b_down, st));
         if (a.bias_part) fin.total[0] = ColumnTotal{a.bias_part, m, 2 * s.hidden, s.hidden, {g.b_gate, g.b_up}};
-    }
-    if (g.b_down) {
-        float* cp = reinterpret_cast<float*>(base + o.dbd);
-        const int64_t units = cdiv(s.n, colsum_rows(s.n));
-        const int lanes = s.c <= 64 ? 8 : (s.c <= 128 ? 16 : 32);
-        colsum_kernel<<<dim3(static_cast<unsigned>(units), static_cast<unsigned>(cdiv(s.c, 8 * lanes))), 256, 0, st>>>(
-            dy, s.n, s.c, bf, lanes, colsum_rows(s.n), cp);
-        MSC_TRY(cudaGetLastError());
-        fin.total[1] = ColumnTotal{cp, units, s.c, s.c, {g.b_down, nullptr}};
     }
     if (g.dx) {
         FfnGemmArgs a{};
@@ -495,7 +515,7 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
             a.partial_split = e;
             fin.split[0] = SplitSum{a.partial, e, p.splits, {g.dx, nullptr, nullptr}, {0, e, e, e}, nullptr, s.c};
         }
-        MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, p.cg, st));
+        MSC_TRY(launch_gemm<FFN_DX>(a, p.ht, p.cg, false, st));
     }
     if (g.w_gate) {
         FfnGemmArgs a{};
@@ -523,7 +543,7 @@ cudaError_t launch_ffn_backward(const FfnShape& s, const void* x, const void* dy
             a.partial_split = 3 * ch;
             fin.split[1] = SplitSum{a.partial, 3 * ch, p.splits, {om[0], om[1], om[2]}, {0, ch, 2 * ch, 3 * ch}, nullptr, s.c};
         }
-        MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, p.cg, st));
+        MSC_TRY(launch_gemm<FFN_DW>(a, p.ht, p.cg, false, st));
     }
     return launch_finish(fin, st);
 }

@@ -511,6 +511,8 @@ __global__ void __launch_bounds__(FfnCfg<MODE, HT, CG>::THREADS, 1) ffn_gemm_ker
     S.tmem = reinterpret_cast<uint32_t*>(S.drained + 1);
     S.abort = reinterpret_cast<int*>(S.tmem + 1);
 
+    // the next kernel of the pass may set itself up on SMs that fall idle
+    launch_dependents();
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -542,6 +544,9 @@ __global__ void __launch_bounds__(FfnCfg<MODE, HT, CG>::THREADS, 1) ffn_gemm_ker
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *S.tmem;
+    // nothing of the kernels before is read, and nothing they read is
+    // written, until they are done
+    wait_dependency();
 
     if (warp == 0) {
         if ((threadIdx.x & 31) == 0) ffn_producer<MODE, HT, CG>(a, S, rank);
