@@ -567,8 +567,8 @@ typedef struct {
 size_t msc_gated_ffn_workspace_bytes(int64_t n, int c, int hidden);
 
 /* Accumulation, activation and gating are fp32; the hidden values are
- * rounded once to the features' type (the tensor cores' operand).  y may be
- * x. */
+ * rounded once to the features' type (the tensor cores' operand; in fp16
+ * they overflow beyond 65504, as any fp16 value).  y may be x. */
 int msc_gated_ffn(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, void* y, void* ws,
                   size_t ws_bytes, void* stream);
 

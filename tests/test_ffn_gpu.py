@@ -410,6 +410,30 @@ def test_stack_is_the_operators_in_turn(ex):
     assert torch.equal(buf[:513], x) and (buf[513:] == 7.0).all()
 
 
+@pytest.mark.parametrize("x_dtype", [torch.float32, torch.bfloat16])
+def test_stack_of_post_norm_blocks(ex, x_dtype):
+    """Blocks without a pre norm (the block sees the stream in its own type)
+    and without a gate.  The stream is rounded to 16 bits before each block
+    (u), the hidden values and the branch once each: 3 u a block of a branch of
+    order one on a stream of order one, 2 blocks, plus the 16-bit stream's."""
+    x, blocks, _ = make_stack(80, 333, 72, 136, torch.bfloat16, 0)
+    blocks = [{**b, "pre": None, "gate": None, "res_scale": 1.0,
+               "post": dict(kind="layer", w=None, b=None, eps=1e-6)} for b in blocks[:2]]
+    x = x.to(x_dtype)
+    want = x.double()
+    for b in blocks:
+        w = {k: v.double() for k, v in b["ffn"].items()}
+        h = want
+        g, u = h @ w["w_gate"].T + w.get("b_gate", 0.0), h @ w["w_up"].T + w.get("b_up", 0.0)
+        want = want + norm64(act64(g, b["act"])[0] * u @ w["w_down"].T + w.get("b_down", 0.0), b["post"])
+    got = ex.ffn_stack(x.clone(), blocks)
+    ex.check()
+    rel = ((got.double() - want).norm() / want.norm()).item()
+    # a relative error of the branch's input passes through the block with a
+    # factor of at most two (gate and up each carry it once)
+    assert rel <= 2 * 2 * 3 * 2.0 ** -8, rel
+
+
 def test_stack_refused_before_it_starts(ex):
     x, blocks, coords = make_stack(60, 40, 64, 128, torch.bfloat16, 2)
     before = x.clone()
