@@ -446,3 +446,26 @@ def test_stack_refused_before_it_starts(ex):
     assert torch.equal(x, before)
     assert ex.ffn_stack(x, []) is x
     assert ex.ffn_stack(x[:0].contiguous(), blocks, coords=coords[:0].contiguous()).shape == (0, 64)
+
+
+@pytest.mark.parametrize("n,c,hidden", [(16900000, 128, 64), (8500000, 256, 64)])
+def test_offsets_past_32_bits(ex, n, c, hidden):
+    """More than 2^31 elements: the last rows, and rows around the 2^31st
+    element, of the single kernel, the CTA pairs and the backward pass."""
+    _, _, ffn = make(90, 1, c, hidden, torch.bfloat16, True)
+    x = torch.empty(n, c, dtype=torch.bfloat16, device="cuda").normal_()
+    picks = [slice(0, 200), slice(2 ** 31 // c - 100, 2 ** 31 // c + 100), slice(n - 200, n)]
+    y = ex.gated_ffn(x, ffn)
+    ex.check()
+    for p in picks:
+        want, bound = fwd_bound(x[p], ffn, "silu", torch.bfloat16)
+        check(y[p], want, bound, f"y {p}")
+    del y
+    if c == 256:
+        dy = torch.empty_like(x).normal_()
+        got = ex.gated_ffn_backward(x, dy, ffn, weights=False)
+        ex.check()
+        for p in picks:
+            want, bound = bwd_reference(x[p], dy[p], ffn, "silu", torch.bfloat16)
+            check(got["x"][p], want["x"], bound["x"], f"dx {p}")
+    torch.cuda.empty_cache()

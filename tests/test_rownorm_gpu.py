@@ -348,3 +348,31 @@ def test_refusals(ex):
     with pytest.raises(MscError, match="no gradient"):
         ex.residual_norm_backward(x, f, None, None)
     assert ex.check() == 0
+
+
+def test_offsets_past_32_bits(ex):
+    """More than 2^31 elements: rows at the start, around the 2^31st element
+    and at the end, and a column sum over all of them."""
+    n, c = 34000000, 64
+    _, _, _, _, cfg = make(40, 1, c, torch.bfloat16, torch.bfloat16, "rms", "layer", "channel")
+    x = torch.empty(n, c, dtype=torch.bfloat16, device="cuda").normal_()
+    f = torch.empty_like(x).normal_()
+    picks = [slice(0, 100), slice(2 ** 31 // c - 50, 2 ** 31 // c + 50), slice(n - 100, n)]
+    r, h = ex.residual_norm(x, f, **cfg)
+    ex.check()
+    for p in picks:
+        wr, wh = forward64(x[p], f[p], cfg, 1.0)
+        close(r[p], wr, c, f"r {p}")
+        close(h[p], wh, c, f"h {p}")
+    got = ex.residual_norm_backward(x, f, r, h, **cfg)
+    ex.check()
+    for p in picks:
+        want, _ = backward64(x[p], f[p], r[p], h[p], cfg, 1.0)
+        for k in ("x", "f"):
+            close(got[k][p], want[k], c, f"{k} {p}", extra=(c + 32) * F32)
+    total = sum(h[i:i + 1000000].double().sum(0) for i in range(0, n, 1000000))
+    size = sum(h[i:i + 1000000].double().abs().sum(0) for i in range(0, n, 1000000))
+    # a warp adds ~14,000 rows in fp32 (each addition 2^-24 of the sum so far,
+    # which grows like the root of the rows), then double
+    assert ((got["pre_b"].double() - total).abs() <= 14500 * 2.0 ** -24 * size).all()
+    torch.cuda.empty_cache()
