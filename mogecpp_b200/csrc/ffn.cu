@@ -49,9 +49,11 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Tile of a product with `cols` output columns: pairs of CTAs on 256 rows
-// where every pair of SMs gets one, else the widest column tile that still
-// gives every SM a tile (wider tiles read less shared memory per product;
-// narrower ones spread few rows over more SMs).
+// where every pair of SMs gets one, else the widest column tile that gives
+// half the SMs one (wider tiles read less shared memory per product; narrower
+// ones spread few rows over more SMs).  Measured with half / all of the SMs as
+// the rule (us, whole block): 1,237 rows of 1024 -> 1376 23.0 / 27.8, 3,000 of
+// 512 -> 2048 33.7 / 41.2; backward 1,237 of 1024 -> 1376 60.2 / 69.2.
 struct TilePlan {
     int ht, cg;
 };
@@ -60,7 +62,7 @@ TilePlan tile_plan(int64_t rows, int cols) {
     for (int ht = 256; ht > 64; ht /= 2) {
         if (cols <= ht / 2) continue;
         if (pairs * cdiv(cols, ht) >= kSms / 2) return {ht, 2};
-        if (m * cdiv(cols, ht) >= kSms) return {ht, 1};
+        if (m * cdiv(cols, ht) >= kSms / 2) return {ht, 1};
     }
     return {64, 1};
 }
@@ -406,9 +408,11 @@ cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, vo
     const int64_t m = cdiv(s.n, 128);
     {
         FfnGemmArgs a{};
-        // pairs on 256 rows x 128 hidden units, as tile_plan
+        // pairs on 256 rows x 128 hidden units, as tile_plan; below, the wide
+        // tile while half the SMs get one (us, 128 / 64 columns: 300 rows of
+        // 1024 -> 4096 24.4 / 26.8, 1,237 of 1024 -> 1376 27.6 / 29.5)
         const int cg = cdiv(s.n, 256) * cdiv(s.hidden, 128) >= kSms / 2 ? 2 : 1;
-        const int ht = cg == 2 || m * cdiv(s.hidden, 128) >= kSms ? 128 : 64;
+        const int ht = cg == 2 || m * cdiv(s.hidden, 128) >= kSms / 2 ? 128 : 64;
         MSC_TRY(make_map_16bit(&a.ma[0], x, bf, s.n, s.c, 128));
         MSC_TRY(make_map_16bit(&a.mb[0], w.w_gate, bf, s.hidden, s.c, ht));
         MSC_TRY(make_map_16bit(&a.mb[1], w.w_up, bf, s.hidden, s.c, ht));

@@ -4,8 +4,8 @@
 //
 // Output tiles of 128 rows x HT columns of a CTA, or of 256 rows of a CTA
 // pair (CG = 2: tcgen05's cta_group::2, each CTA holding its own 128 rows of
-// A and half of B's, which halves B's copies and shared-memory reads); the K loop runs in steps of 64
-// elements through a ring of shared-memory stages filled by TMA (128-byte
+// A and half of B's, which halves B's copies and shared-memory reads); the K
+// loop runs in steps of 64 elements through a ring of shared-memory stages filled by TMA (128-byte
 // swizzle; rows, columns and K past the extents read as zero, so every size
 // that is a multiple of 8 is right without a special case).  Operands that
 // are contiguous along K are K-major; the transposed products of the
