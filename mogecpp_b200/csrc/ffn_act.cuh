@@ -37,11 +37,22 @@ __device__ __forceinline__ uint64_t reciprocal2(uint64_t d) {
     return pack2(r * b, r * a);
 }
 
-// sigma(v) = 1 / (1 + 2^(-v log2 e)).  The exponent is held at 62, where
-// sigma is 2^-62 in place of less: v sigma(v) is then off by |v| 2^-62 at
+// e = 2^(-v log2 e) of sigma(v) = 1 / (1 + e).  The exponent is held at 62,
+// where sigma is 2^-62 in place of less: v sigma(v) is then off by |v| 2^-62 at
 // most.
-__device__ __forceinline__ uint64_t sigmoid2(uint64_t v) {
-    return reciprocal2(add2(exp2_2(min2(mul2(v, both(-1.4426950408889634f)), 62.0f)), both(1.0f)));
+__device__ __forceinline__ uint64_t sigmoid_exp2(uint64_t v) {
+    return exp2_2(min2(mul2(v, both(-1.4426950408889634f)), 62.0f));
+}
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t v) { return reciprocal2(add2(sigmoid_exp2(v), both(1.0f))); }
+
+// sigma(v), and rest = 1 - sigma(v) as e sigma(v): it goes to exactly 0 with e
+// far above zero, where 1 - s would keep the last bits of s (which depend on
+// the lane's neighbour), for the derivatives to multiply by v or more.
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t v, uint64_t& rest) {
+    const uint64_t e = sigmoid_exp2(v);
+    const uint64_t s = reciprocal2(add2(e, both(1.0f)));
+    rest = mul2(e, s);
+    return s;
 }
 
 // GELU's tanh form as g sigma(2 z), z = sqrt(2/pi) (g + 0.044715 g^3): the
@@ -88,20 +99,29 @@ __device__ __forceinline__ uint64_t act_value(uint64_t g) {
     }
 }
 
-// Activation v and its derivative dv.
+// GELU's derivative takes its polynomials at min(g, 15): from there on e is
+// exactly 0 (2^-380), and g^3 stays finite.
+__device__ __forceinline__ uint64_t gelu_ceiling2(uint64_t g) {
+    float a, b;
+    unpack2(g, a, b);
+    return pack2(a > 15.0f ? 15.0f : a, b > 15.0f ? 15.0f : b);
+}
+
+// Activation v and its derivative dv: s + v (1 - s) (slope of sigma's argument).
 template <int ACT>
 __device__ __forceinline__ void act_both(uint64_t g, uint64_t& v, uint64_t& dv) {
-    const uint64_t one = both(1.0f), minus = both(-1.0f);
     if constexpr (ACT == ACT_SILU) {
-        const uint64_t s = sigmoid2(g);
+        uint64_t rest;
+        const uint64_t s = sigmoid2(g, rest);
         v = mul2(g, s);
-        dv = fma2(v, fma2(s, minus, one), s);
+        dv = fma2(v, rest, s);
     } else if constexpr (ACT == ACT_GELU) {
         g = gelu_floor2(g);
-        const uint64_t gg = mul2(g, g);
-        const uint64_t s = sigmoid2(mul2(g, fma2(gg, both(kGelu1), both(kGelu0))));
+        const uint64_t gc = gelu_ceiling2(g), gg = mul2(gc, gc);
+        uint64_t rest;
+        const uint64_t s = sigmoid2(mul2(gc, fma2(gg, both(kGelu1), both(kGelu0))), rest);
         v = mul2(g, s);
-        dv = fma2(mul2(v, fma2(s, minus, one)), fma2(gg, both(3.0f * kGelu1), both(kGelu0)), s);
+        dv = fma2(mul2(v, rest), fma2(gg, both(3.0f * kGelu1), both(kGelu0)), s);
     } else {
         uint64_t gauss;
         const uint64_t p = normal_cdf2(g, gauss);

@@ -1,0 +1,74 @@
+"""Feed-forward blocks at the edges of their range: gates far from zero beside
+ordinary ones, stacks of mixed hidden sizes, long sums, calls in place.  The
+64-bit formulas and the bound of an element are those of test_ffn_gpu."""
+import math
+
+import pytest
+import torch
+
+from test_ffn_gpu import act64, bwd_reference, check, fwd_bound, make
+
+pytestmark = pytest.mark.gpu
+
+F32 = 2.0 ** -23
+
+
+def at_gates(ex, g, act):
+    """act(g) and act'(g) in fp32, through the public backward pass: one row
+    with dh = 1 and up = 1, whose gates are the bias itself, has db_gate =
+    act'(g) and db_up = act(g), both unrounded."""
+    hidden = g.numel()
+    zero = torch.zeros(hidden, 8, device="cuda", dtype=torch.bfloat16)
+    ffn = dict(w_gate=zero, w_up=zero, w_down=torch.ones(8, hidden, device="cuda", dtype=torch.bfloat16),
+               b_gate=g, b_up=torch.ones(hidden, device="cuda"))
+    x = torch.zeros(1, 8, device="cuda", dtype=torch.bfloat16)
+    dy = x.clone()
+    dy[0, 0] = 1.0
+    got = ex.gated_ffn_backward(x, dy, ffn, act=act)
+    ex.check()
+    return got["b_up"].double(), got["b_gate"].double()
+
+
+def gate_slope64(g, act):
+    """sigma's argument of the activation, its slope and exponent (64 bits)."""
+    if act == "silu":
+        return torch.ones_like(g), g / math.log(2)
+    k = 2 * math.sqrt(2 / math.pi)
+    return k * (1 + 3 * 0.044715 * g * g), k * (g + 0.044715 * g ** 3) / math.log(2)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_erf"])
+@pytest.mark.parametrize("far", [6.0, 10.0, 30.0, 100.0, 1e3, 1e4, 3e5, 1e10, 1e30])
+def test_large_gates_beside_ordinary_ones(ex, act, far):
+    """Two neighbouring units share a reciprocal: the derivative at a large
+    gate is one whatever stands beside it, and the neighbour's is its own.
+
+    dv = s + v (1 - s) slope in fp32: s within 4 units in the last place; e =
+    2^a, of which 1 - s = e s is made, within (4 + 2 |a|) units (the argument's
+    two roundings and ex2's error, in units of a; counted up to a = 126, beyond
+    which e is zero on both sides but for 2^-126); v and the slope within 4
+    each.  The erf form's e^(-g^2 / 2) and polynomial: 1.5e-7 in erf, and the
+    density's (8 + g^2) units."""
+    partners = torch.linspace(-3.0, 3.0, 4096, device="cuda")
+    for flip in (False, True):
+        pair = [torch.full_like(partners, far), partners]
+        g = torch.stack(pair[::-1] if flip else pair, 1).reshape(-1).contiguous()
+        v, dv = at_gates(ex, g, act)
+        g = g.double()
+        if act == "gelu_erf":
+            want_v, want_dv = act64(g, act)
+            density = torch.exp(-g * g / 2) * g.abs()
+            bound_v = 2e-7 * g.abs().clamp(max=6.0) + 8 * F32 * want_v.abs()
+            bound_dv = 1e-7 + 8 * F32 + (8 + g * g) * F32 * density
+        else:
+            # tanh of a number this large is one, and 1 - s zero, in 64 bits too
+            gc = g.clamp(max=40.0)
+            slope, a = gate_slope64(gc, act)
+            s = torch.sigmoid(a * math.log(2))
+            rest = torch.sigmoid(-a * math.log(2))
+            want_v, want_dv = g * s, s + gc * s * rest * slope
+            bound_v = (8 + 2 * a.abs().clamp(max=126) * rest) * F32 * want_v.abs() + 1e-30
+            bound_dv = 8 * F32 * s + (16 + 2 * a.abs().clamp(max=126)) * F32 * (gc * s * rest * slope).abs() + 1e-30
+        assert v.isfinite().all() and dv.isfinite().all()
+        worst = ((v - want_v).abs() / bound_v).max().item(), ((dv - want_dv).abs() / bound_dv).max().item()
+        assert worst[0] <= 1.0 and worst[1] <= 1.0, (act, far, worst)
