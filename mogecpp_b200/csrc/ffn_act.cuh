@@ -39,7 +39,8 @@ __device__ __forceinline__ uint64_t reciprocal2(uint64_t d) {
 
 // e = 2^(-v log2 e) of sigma(v) = 1 / (1 + e).  The exponent is held at 62,
 // where sigma is 2^-62 in place of less: v sigma(v) is then off by |v| 2^-62 at
-// most.
+// most, so that the activations hold their gates where that is nothing
+// (floor2).  NaN comes out as the floor too, and leaves the neighbour alone.
 __device__ __forceinline__ uint64_t sigmoid_exp2(uint64_t v) {
     return exp2_2(min2(mul2(v, both(-1.4426950408889634f)), 62.0f));
 }
@@ -60,13 +61,29 @@ __device__ __forceinline__ uint64_t sigmoid2(uint64_t v, uint64_t& rest) {
 constexpr float kGelu0 = 1.5957691216057308f;   // 2 sqrt(2/pi)
 constexpr float kGelu1 = 0.07135481282553484f;  // 2 sqrt(2/pi) 0.044715
 
-// g held at -15, below which GELU and its derivative are under 2^-300: sigma's
-// floor times the cube in the derivative would grow again far out.  NaN stays.
-__device__ __forceinline__ uint64_t gelu_floor2(uint64_t g) {
+// The lanes held at m from below / above; NaN stays.
+__device__ __forceinline__ uint64_t floor2(uint64_t v, float m) {
     float a, b;
-    unpack2(g, a, b);
-    return pack2(a < -15.0f ? -15.0f : a, b < -15.0f ? -15.0f : b);
+    unpack2(v, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(m));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(m));
+    return pack2(a, b);
 }
+__device__ __forceinline__ uint64_t ceiling2(uint64_t v, float m) {
+    float a, b;
+    unpack2(v, a, b);
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(m));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(m));
+    return pack2(a, b);
+}
+
+// Gates are held where sigma reaches its floor and the activation and its
+// derivative are under 2^-55 (SiLU; 2^-300 GELU): further out the floor times
+// the gate, or GELU's cube, would grow again.
+constexpr float kSiluFloor = -43.0f, kGeluFloor = -15.0f;
+// GELU's derivative takes its polynomials at min(g, 15): from there on e is
+// exactly 0 (2^-380), and g^3 stays finite.
+constexpr float kGeluCeiling = 15.0f;
 
 // Phi(g) = (1 + erf(g / sqrt 2)) / 2 by Abramowitz and Stegun's 7.1.26
 // (|error| <= 1.5e-7 in erf): erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2), t =
@@ -89,9 +106,10 @@ __device__ __forceinline__ uint64_t normal_cdf2(uint64_t g, uint64_t& gauss) {
 template <int ACT>
 __device__ __forceinline__ uint64_t act_value(uint64_t g) {
     if constexpr (ACT == ACT_SILU) {
+        g = floor2(g, kSiluFloor);
         return mul2(g, sigmoid2(g));
     } else if constexpr (ACT == ACT_GELU) {
-        g = gelu_floor2(g);
+        g = floor2(g, kGeluFloor);
         return mul2(g, sigmoid2(mul2(g, fma2(mul2(g, g), both(kGelu1), both(kGelu0)))));
     } else {
         uint64_t gauss;
@@ -99,25 +117,18 @@ __device__ __forceinline__ uint64_t act_value(uint64_t g) {
     }
 }
 
-// GELU's derivative takes its polynomials at min(g, 15): from there on e is
-// exactly 0 (2^-380), and g^3 stays finite.
-__device__ __forceinline__ uint64_t gelu_ceiling2(uint64_t g) {
-    float a, b;
-    unpack2(g, a, b);
-    return pack2(a > 15.0f ? 15.0f : a, b > 15.0f ? 15.0f : b);
-}
-
 // Activation v and its derivative dv: s + v (1 - s) (slope of sigma's argument).
 template <int ACT>
 __device__ __forceinline__ void act_both(uint64_t g, uint64_t& v, uint64_t& dv) {
     if constexpr (ACT == ACT_SILU) {
+        g = floor2(g, kSiluFloor);
         uint64_t rest;
         const uint64_t s = sigmoid2(g, rest);
         v = mul2(g, s);
         dv = fma2(v, rest, s);
     } else if constexpr (ACT == ACT_GELU) {
-        g = gelu_floor2(g);
-        const uint64_t gc = gelu_ceiling2(g), gg = mul2(gc, gc);
+        g = floor2(g, kGeluFloor);
+        const uint64_t gc = ceiling2(g, kGeluCeiling), gg = mul2(gc, gc);
         uint64_t rest;
         const uint64_t s = sigmoid2(mul2(gc, fma2(gg, both(kGelu1), both(kGelu0))), rest);
         v = mul2(g, s);

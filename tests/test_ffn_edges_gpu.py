@@ -72,3 +72,25 @@ def test_large_gates_beside_ordinary_ones(ex, act, far):
         assert v.isfinite().all() and dv.isfinite().all()
         worst = ((v - want_v).abs() / bound_v).max().item(), ((dv - want_dv).abs() / bound_dv).max().item()
         assert worst[0] <= 1.0 and worst[1] <= 1.0, (act, far, worst)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_erf"])
+def test_gates_far_below_zero(ex, act):
+    """Far below zero the value and the derivative are nothing, however far:
+    SiLU ends at 43 2^-62 < 1e-17 (its exact value there is 9e-18), GELU below,
+    the erf form at the 1.5e-7 / 2 |g| of its polynomial at most and at exactly
+    zero from 20 on.  The neighbour's are its own, beside NaN and infinity too."""
+    partners = torch.linspace(-3.0, 3.0, 512, device="cuda")
+    alone = at_gates(ex, partners, act)
+    for far in (-45.0, -60.0, -300.0, -1e4, -1e10, -1e20, -1e30, -3e38, float("-inf"), float("inf"), float("nan")):
+        g = torch.stack([torch.full_like(partners, far), partners], 1).reshape(-1).contiguous()
+        v, dv = at_gates(ex, g, act)
+        if math.isfinite(far):
+            assert v[::2].abs().max() <= 1e-17 and dv[::2].abs().max() <= 1e-15, far
+        if math.isnan(far):
+            assert v[::2].isnan().all() and dv[::2].isnan().all()
+        # a reciprocal shared with another partner: a few units in the last
+        # place (of one half in the erf form's distribution function)
+        near = 8 * F32 * alone[0].abs() + (4 * F32 * partners.abs() if act == "gelu_erf" else 0.0) + 1e-30
+        assert ((v[1::2] - alone[0]).abs() <= near).all(), far
+        assert ((dv[1::2] - alone[1]).abs() <= 16 * F32).all(), far
