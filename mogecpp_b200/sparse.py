@@ -490,6 +490,9 @@ class SparseCudaExecutor:
             self._need(gate, name, (c,))
             return 0
         self._need(gate, name, (gate.shape[0], c))
+        if gate.shape[0] == 0 and n > 0:
+            # its address would read as "no gate", its samples as "one gate for all"
+            raise L.MscError(L.MSC_E_INVALID, f"a {name} per sample needs at least one sample")
         if coords is None:
             raise L.MscError(L.MSC_E_INVALID, f"a {name} per sample needs the coordinates")
         self._need(coords, "coords", (n, 4), (torch.int32,))
