@@ -1141,7 +1141,8 @@ int msc_gated_ffn_backward(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, 
         const bool w_any = grads->w_gate || grads->w_up || grads->w_down;
         need(!w_any || (grads->w_gate && grads->w_up && grads->w_down),
              "the weight gradients are asked for together or not at all");
-        need(grads->dx || w_any || grads->b_gate || grads->b_up || grads->b_down, "no gradient asked for");
+        // (an empty dx has no address)
+        need(n == 0 || grads->dx || w_any || grads->b_gate || grads->b_up || grads->b_down, "no gradient asked for");
         need_aligned(grads->dx, 16, "dx");
         need_aligned(grads->w_gate, 16, "w_gate gradient");
         need_aligned(grads->w_up, 16, "w_up gradient");

@@ -94,3 +94,19 @@ def test_gates_far_below_zero(ex, act):
         near = 8 * F32 * alone[0].abs() + (4 * F32 * partners.abs() if act == "gelu_erf" else 0.0) + 1e-30
         assert ((v[1::2] - alone[0]).abs() <= near).all(), far
         assert ((dv[1::2] - alone[1]).abs() <= 16 * F32).all(), far
+
+
+def test_no_rows(ex):
+    """Every call without rows: an empty dx alone, and a gate of no samples
+    where there is no row to look one up."""
+    x, dy, ffn = make(5, 8, 64, 128, torch.bfloat16, True)
+    none = x[:0].contiguous()
+    got = ex.gated_ffn_backward(none, none, ffn, weights=False)
+    assert set(got) == {"x"} and got["x"].shape == (0, 64)
+    gate, coords = torch.zeros(0, 64, device="cuda"), torch.zeros(0, 4, dtype=torch.int32, device="cuda")
+    r, h = ex.residual_norm(none, none, gate=gate, coords=coords, pre=dict(kind="rms", eps=1e-6))
+    assert r.shape == h.shape == (0, 64)
+    got = ex.residual_norm_backward(none, none, none, none, gate=gate, coords=coords, pre=dict(kind="rms", eps=1e-6))
+    assert got["gate"].shape == (0, 64) and got["x"].shape == got["f"].shape == (0, 64)
+    assert ex.ffn_stack(none, [dict(ffn=ffn, gate=gate)], coords=coords) is none
+    assert ex.check() == 0
