@@ -601,7 +601,8 @@ typedef struct {
 
 /* nblocks residual feed-forward blocks in a row, in place on x (a level's
  * block loop in one call, beside msc_res_stack): each block's exit and the
- * next block's entry norm are one pass.  Workspace: of the largest hidden. */
+ * next block's entry norm are one pass.  Workspace: of the largest hidden (the
+ * query never shrinks as hidden grows). */
 size_t msc_ffn_stack_workspace_bytes(int64_t n, int c, int hidden);
 int msc_ffn_stack(msc_ctx_t ctx, void* x, int x_dtype, int64_t n, int c, const int32_t* coords, int nsamples,
                   int nblocks, const msc_ffn_block* blocks, void* ws, size_t ws_bytes, void* stream);

@@ -1164,7 +1164,7 @@ int msc_gated_ffn_backward(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, 
 
 size_t msc_ffn_stack_workspace_bytes(int64_t n, int c, int hidden) {
     if (!ffn_sizes_ok(n, c, hidden)) return 0;
-    return 2 * align256(static_cast<size_t>(n) * c * 2) + align256(msc::ffn_workspace_bytes(n, c, hidden));
+    return 2 * align256(static_cast<size_t>(n) * c * 2) + align256(msc::ffn_workspace_bound(n, c, hidden));
 }
 
 int msc_ffn_stack(msc_ctx_t ctx, void* x, int x_dtype, int64_t n, int c, const int32_t* coords, int nsamples,

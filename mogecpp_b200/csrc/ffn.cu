@@ -67,10 +67,17 @@ TilePlan tile_plan(int64_t rows, int cols) {
     return {64, 1};
 }
 
-// Splits of a K of `ksteps` steps when `tiles` output tiles leave SMs idle.
-int k_splits(int64_t tiles, int ksteps, int min_steps, int* ksplit) {
-    int64_t s = tiles > 0 && tiles * 2 <= kSms ? kSms / tiles : 1;
-    s = std::max<int64_t>(1, std::min<int64_t>(s, ksteps / min_steps));
+// Splits of a K of `ksteps` steps when `tiles` output tiles leave SMs idle, of
+// at least kMinSteps steps each.  The splits of equal length that K is then cut
+// into may be fewer (24 steps: 6 of 4; 25: 5 of 5); the most there may be grows
+// with K.
+constexpr int kMinSteps = 4;
+int most_splits(int64_t tiles, int ksteps) {
+    const int64_t s = tiles > 0 && tiles * 2 <= kSms ? kSms / tiles : 1;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(s, ksteps / kMinSteps)));
+}
+int k_splits(int64_t tiles, int ksteps, int* ksplit) {
+    const int s = most_splits(tiles, ksteps);
     ksteps = std::max(ksteps, 1);
     *ksplit = static_cast<int>(cdiv(ksteps, s));
     return static_cast<int>(cdiv(ksteps, *ksplit));
@@ -82,7 +89,7 @@ struct ProjPlan {
 ProjPlan proj_plan(int64_t n, int cols, int ksteps) {
     const TilePlan t = tile_plan(n, cols);
     ProjPlan p{t.ht, t.cg, 1, ksteps};
-    if (t.cg == 1) p.splits = k_splits(cdiv(n, 128) * cdiv(cols, p.ht), ksteps, 4, &p.ksplit);
+    if (t.cg == 1) p.splits = k_splits(cdiv(n, 128) * cdiv(cols, p.ht), ksteps, &p.ksplit);
     return p;
 }
 
@@ -101,7 +108,7 @@ DwPlan dw_plan(int64_t n, int c, int hidden) {
     const int ksteps = static_cast<int>(cdiv(n, 64));
     p.splits = 1;
     p.ksplit = std::max(ksteps, 1);
-    if (p.cg == 1) p.splits = k_splits(p.tiles, ksteps, 4, &p.ksplit);
+    if (p.cg == 1) p.splits = k_splits(p.tiles, ksteps, &p.ksplit);
     // no sum in one accumulator runs over more than 32768 rows: the tensor
     // core's fp32 accumulator truncates, a drift that grows with the chain
     if (p.ksplit > 512) {
@@ -394,6 +401,19 @@ cudaError_t make_map_16bit(CUtensorMap* map, const void* base, bool bf16, int64_
 }
 
 size_t ffn_workspace_bytes(int64_t n, int c, int hidden) { return fwd_ws(n, c, hidden).total; }
+
+size_t ffn_workspace_bound(int64_t n, int c, int hidden) {
+    if (use_fused(n, c)) return 0;
+    // the dot products' fp32 hidden values end at a size (ffn_few_rows)
+    int few = hidden / 8 * 8;
+    if (!ffn_few_rows(n, c, few)) few = ffn_few_rows(n, c, 8) ? static_cast<int>(kFewRowsWork / (n * c) / 8 * 8) : 0;
+    const size_t rows = align256(static_cast<size_t>(n) * few * 4);
+    if (few >= hidden) return rows;
+    const TilePlan t = tile_plan(n, c);
+    const int splits = t.cg == 1 ? most_splits(cdiv(n, 128) * cdiv(c, t.ht), static_cast<int>(cdiv(hidden, 64))) : 1;
+    const size_t part = splits > 1 ? align256(static_cast<size_t>(splits) * n * c * 4) : 0;
+    return std::max(rows, align256(static_cast<size_t>(n) * hidden * 2) + part);
+}
 size_t ffn_backward_workspace_bytes(int64_t n, int c, int hidden) { return bwd_ws(n, c, hidden).total; }
 
 cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, void* y, void* ws, uint32_t* status,

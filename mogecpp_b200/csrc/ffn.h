@@ -38,6 +38,9 @@ struct FfnGrads {
 };
 
 size_t ffn_workspace_bytes(int64_t n, int c, int hidden);
+// Enough for every block of at most `hidden` hidden units (the size itself
+// shrinks here and there as hidden grows: fewer K splits, or another path).
+size_t ffn_workspace_bound(int64_t n, int c, int hidden);
 cudaError_t launch_ffn(const FfnShape& s, const void* x, const FfnWeights& w, void* y, void* ws, uint32_t* status,
                        cudaStream_t st);
 size_t ffn_backward_workspace_bytes(int64_t n, int c, int hidden);

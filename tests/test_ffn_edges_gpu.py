@@ -110,3 +110,18 @@ def test_no_rows(ex):
     assert got["gate"].shape == (0, 64) and got["x"].shape == got["f"].shape == (0, 64)
     assert ex.ffn_stack(none, [dict(ffn=ffn, gate=gate)], coords=coords) is none
     assert ex.check() == 0
+
+
+@pytest.mark.parametrize("n,c,sizes", [(300, 512, (1536, 1600)), (64, 256, (1600, 1536)), (8, 128, (16384, 16392))])
+def test_stack_of_mixed_hidden_sizes(ex, n, c, sizes):
+    """Blocks of which the smaller one needs the larger workspace, in one
+    call: the operators in turn, bit for bit."""
+    nrm = dict(kind="rms", eps=1e-6)
+    blocks = [dict(ffn=make(i, 1, c, h, torch.bfloat16, True)[2], pre=nrm) for i, h in enumerate(sizes)]
+    x = make(9, n, c, 8, torch.bfloat16, False)[0].float()
+    want, h = ex.residual_norm(x, pre=nrm, branch_dtype=torch.bfloat16)
+    for i, b in enumerate(blocks):
+        want, h = ex.residual_norm(want, ex.gated_ffn(h, b["ffn"]), pre=nrm if i == 0 else None)
+    got = ex.ffn_stack(x.clone(), blocks)
+    ex.check()
+    assert torch.equal(got, want)

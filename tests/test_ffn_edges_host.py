@@ -29,3 +29,22 @@ def test_gate_of_no_samples_is_refused(host_ex):
                  lambda: host_ex.ffn_stack(x, [dict(ffn=ffn, gate=gate)], coords=coords)):
         with pytest.raises(L.MscError, match="at least one sample"):
             call()
+
+
+@pytest.mark.parametrize("n", [1, 4, 5, 8, 9, 64, 128, 300, 1237, 4736, 18943, 18944])
+@pytest.mark.parametrize("c", [8, 64, 128, 256, 512, 1024, 8192])
+def test_stack_workspace_covers_smaller_blocks(n, c):
+    """A stack's workspace is asked for with the largest hidden size: it holds
+    every smaller block's, though a block of its own may need less as it grows
+    (fewer K splits, or another path)."""
+    lib = L.load()
+    rows = 2 * ((n * c * 2 + 255) // 256 * 256)
+    most = 0
+    for hidden in [*range(8, 4200, 8), *range(4200, 65536, 1000), 65536]:
+        most = max(most, rows + lib.msc_gated_ffn_workspace_bytes(n, c, hidden))
+        assert lib.msc_ffn_stack_workspace_bytes(n, c, hidden) >= most, hidden
+    # around the end of the dot products (8 rows of 128 channels: 16,384 hidden units)
+    size = [lib.msc_ffn_stack_workspace_bytes(n, c, h) for h in range(8, 65537, 8)]
+    assert all(a <= b for a, b in zip(size, size[1:]))
+    # no more than the splits' own rounding costs
+    assert size[-1] <= 2 * most
