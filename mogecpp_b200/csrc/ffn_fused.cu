@@ -20,6 +20,10 @@
 // and the registers of a third group would cost more than it brings (177 us
 // against 170 at 402,131 x 128 -> 512, bf16), each subtile has a group.
 //
+// Y's chain in its accumulator is the whole hidden size, at most 65,536: not
+// cut at 32,768 as the products of ffn.cu are, since what it then drifts by for
+// terms of one sign stays below half of fp16's rounding.
+//
 // TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 and 2
 // MMA issuers (D, Y), 3 TMEM allocation (and stores), 4 on epilogue (8 per
 // group: lane quarter x half of the chunk).  Every wait is bounded, as in

@@ -125,3 +125,56 @@ def test_stack_of_mixed_hidden_sizes(ex, n, c, sizes):
     got = ex.ffn_stack(x.clone(), blocks)
     ex.check()
     assert torch.equal(got, want)
+
+
+# (rows, channels): CTA pairs of 256 columns, single CTAs, CTA pairs of 128 columns (backward: the forward
+# pass of that many rows and few channels is one kernel, whose chain is the whole hidden size)
+@pytest.mark.parametrize("n,c", [(9500, 1024), (4900, 512), (20000, 128)])
+def test_long_sums_do_not_drift(ex, n, c):
+    """65,536 hidden units, terms of one sign.  A chain of 32,768 elements in
+    one fp32 accumulator drifts by 1.2e-4 of its sum (measured: the tensor core
+    truncates), one of 131,072 (dx in one accumulator) by 4.4e-4; the parts'
+    fp32 additions add 4 2^-24.  The mean over 64 x c outputs takes their 16-bit
+    rounding out (2^-11 / sqrt(3 * 64 c) < 4e-6).  Limit: twice the short
+    chain's drift; the single kernel's chain of 65,536, twice that."""
+    hidden = 65536
+    gen = torch.Generator(device="cuda").manual_seed(n)
+
+    def positive(*shape, scale):
+        return ((1.0 + torch.rand(shape, generator=gen, device="cuda")) * scale).half()
+    # gates of 40: act(g) = 40, act' = 1; h = 1 for y, dg and du one sum of w_down times 1 / 40 and 1 for dx
+    up = torch.full((hidden,), 1 / 40, device="cuda")
+    ffn = dict(w_gate=positive(hidden, c, scale=2.0 ** -8), w_up=positive(hidden, c, scale=2.0 ** -8),
+               w_down=positive(c, hidden, scale=2.0 ** -8), b_gate=torch.full((hidden,), 40.0, device="cuda"), b_up=up)
+    x = torch.zeros(n, c, device="cuda", dtype=torch.float16)
+    y = ex.gated_ffn(x, ffn)
+    ex.check()
+    h = torch.full((hidden,), 40.0 * up[0].double().item(), device="cuda", dtype=torch.float16).double()
+    drift = (y[:64].double() / (ffn["w_down"].double() @ h) - 1).mean().item()
+    assert abs(drift) <= (4.8e-4 if c <= 128 else 2.4e-4), drift
+    dy = torch.full((n, c), 2.0 ** -6, device="cuda", dtype=torch.float16)
+    dx = ex.gated_ffn_backward(x, dy, ffn, weights=False)["x"]
+    ex.check()
+    dh = ffn["w_down"].double().sum(0) * 2.0 ** -6
+    dg, du = (dh * up[0].double()).half().double(), (dh * 40.0).half().double()
+    want = dg @ ffn["w_gate"].double() + du @ ffn["w_up"].double()
+    drift = (dx[:64].double() / want - 1).mean().item()
+    assert abs(drift) <= 2.4e-4, drift
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,c", [(9500, 264), (4900, 512)])
+def test_long_sums(ex, n, c):
+    """The same parts of a long sum on random data, rows of the first and the
+    last tile: every element within its bound, and the same bits again."""
+    x, dy, ffn = make(n, n, c, 65536, torch.bfloat16, True)
+    y = ex.gated_ffn(x, ffn)
+    dx = ex.gated_ffn_backward(x, dy, ffn, weights=False)["x"]
+    ex.check()
+    assert torch.equal(y, ex.gated_ffn(x, ffn))
+    for p in (slice(0, 40), slice(n - 40, n)):
+        want, bound = fwd_bound(x[p], ffn, "silu", torch.bfloat16)
+        check(y[p], want, bound, f"y {p}")
+        want, bound = bwd_reference(x[p], dy[p], ffn, "silu", torch.bfloat16)
+        check(dx[p], want["x"], bound["x"], f"dx {p}")
+    torch.cuda.empty_cache()
