@@ -178,3 +178,30 @@ def test_long_sums(ex, n, c):
         want, bound = bwd_reference(x[p], dy[p], ffn, "silu", torch.bfloat16)
         check(dx[p], want["x"], bound["x"], f"dx {p}")
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,c,hidden", [(40000, 1024, 2048), (40000, 512, 2048), (70000, 72, 200)])
+def test_weight_gradients_of_many_rows(ex, n, c, hidden):
+    """More than 32,768 rows: the weight gradients' sums in two and three
+    parts, on CTA pairs and on single CTAs."""
+    x, dy, ffn = make(n + c, n, c, hidden, torch.bfloat16, True)
+    got = ex.gated_ffn_backward(x, dy, ffn)
+    ex.check()
+    want, bound = bwd_reference(x, dy, ffn, "silu", torch.bfloat16)
+    for k in got:
+        check(got[k], want[k], bound[k], k)
+    again = ex.gated_ffn_backward(x, dy, ffn)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,c,hidden", [(1, 1024, 2048), (7, 128, 344), (300, 264, 520), (19001, 64, 176), (19500, 128, 344),
+                                        (10000, 264, 520)])
+def test_in_place_on_every_path(ex, n, c, hidden):
+    """y is x: the dot products, single CTAs with a K split, the single kernel
+    of either width, CTA pairs."""
+    x, _, ffn = make(n, n, c, hidden, torch.bfloat16, True)
+    want = ex.gated_ffn(x, ffn)
+    y = x.clone()
+    assert ex.gated_ffn(y, ffn, out=y) is y and torch.equal(y, want)
+    ex.check()
