@@ -31,10 +31,11 @@
 // instruction issue at the 16 warps that 128 registers allow).
 //
 // The backward column sums are kept in fp32 registers over a unit's (warp's
-// or block's) run of rows, written once per unit, and added over the units in
+// or block's) run of rows, at most 1,024 steps, written once per unit, and
+// added over the units (and passes over them, where the rows are more) in
 // double in a fixed order by a second kernel: no atomics, the same bits every
-// time.  A per-sample gate adds its sums to the unit's own slab whenever the
-// sample changes (rows are normally sorted by sample; any order is right).
+// time.  A per-sample gate adds its sums (fp32) to the unit's own slab whenever
+// the sample changes (rows are normally sorted by sample; any order is right).
 #include "rownorm.h"
 
 #include "common.cuh"
@@ -43,6 +44,7 @@
 #include <algorithm>
 #include <atomic>
 #include <mutex>
+#include <type_traits>
 
 namespace msc {
 namespace {
@@ -430,8 +432,10 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rown
     if (sub == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (has(v))
-                for (int q = SLAB_POST_W; q < slab_rows; ++q) clear8(q, (t + v * T) * 8);
+            if (has(v)) {
+#pragma unroll 1
+                for (int q = SLAB_POST_W; q < a.slab_clear; ++q) clear8(q, (t + v * T) * 8);
+            }
     }
     if constexpr (T <= 32) __syncwarp();
     uint64_t pre_w[V * 4], gate_w[V * 4];
@@ -699,13 +703,15 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rown
 }
 
 // Column sums over the units, 8 columns (a 32-byte sector) a block, in double
-// and in a fixed order.
-__global__ void __launch_bounds__(1024) slab_sum_kernel(const float* part, int64_t units, int slab_rows, int c,
-                                                        RowNormGrads g) {
+// and in a fixed order, of the slab rows from row0 on.  Of several passes over
+// the rows each adds its sums to `totals` [4][c], which the first one starts
+// (pass 0), and the last one writes the gradients.
+__global__ void __launch_bounds__(1024) slab_sum_kernel(const float* part, int64_t units, int slab_rows, int row0, int c,
+                                                        double* totals, int64_t pass, bool last, RowNormGrads g) {
     __shared__ double red[128][9];
     const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
     const int col = blockIdx.x * 8 + tx;
-    const int srow = blockIdx.y;
+    const int srow = row0 + blockIdx.y;
     float* dst = nullptr;
     if (srow == SLAB_PRE_W) dst = g.pre_w;
     else if (srow == SLAB_PRE_B) dst = g.pre_b;
@@ -722,7 +728,12 @@ __global__ void __launch_bounds__(1024) slab_sum_kernel(const float* part, int64
         if (ty < o) red[ty][tx] += red[ty + o][tx];
         __syncthreads();
     }
-    if (ty == 0) dst[col] = static_cast<float>(red[0][tx]);
+    if (ty == 0) {
+        double* total = totals + static_cast<int64_t>(srow) * c + col;
+        const double sum = pass ? *total + red[0][tx] : red[0][tx];
+        if (last) dst[col] = static_cast<float>(sum);
+        else *total = sum;
+    }
 }
 
 int sm_count() {
@@ -747,20 +758,35 @@ int row_threads(int c) {
 }
 
 // Units of the backward pass: enough to fill the GPU, at least four steps of
-// rows each where there are that many, and few enough that the slabs stay
-// within 64 MiB however many samples have a gate.
-void backward_units(int64_t n, int c, int nsamples, int64_t* units, int64_t* rows_per_unit) {
+// rows each where there are that many; but no more than 64 MiB of slabs, since
+// a gate per sample takes nsamples rows of each unit's.  Many samples therefore
+// leave fewer units, and the pass slows down: 400,000 x 128 bf16 takes 147 us
+// with 2 samples, 242 with 64, 1,015 with 512, 7,860 with 4,096 and 91,000 with
+// 32,768.
+//
+// No unit's fp32 sums run over more than kRunSteps steps (an fp32 chain over
+// the 100,000 rows that each of three units has left in the last of these was
+// off by 3.5e-4 of a sum of one sign): more rows take several passes.
+constexpr int kRunSteps = 1024;
+struct BackwardPlan {
+    int64_t units, rows_per_unit, passes;
+};
+BackwardPlan backward_plan(int64_t n, int c, int nsamples) {
     const int t = row_threads(c);
     const int64_t r = t > 32 ? 1 : 32 / t;
     constexpr int64_t kSms = 148;  // B200; a fixed count keeps the workspace size and the sums the same everywhere
     int64_t u = t > 32 ? kSms * (512 / t) : kSms * 16;
-    const int64_t slab = static_cast<int64_t>(4 + std::max(nsamples, 1)) * c * 4;
+    const int64_t slab = static_cast<int64_t>(SLAB_GATE + std::max(nsamples, 1)) * c * 4;
     u = std::min(u, std::max<int64_t>((int64_t(64) << 20) / slab, 1));
     u = std::min(u, std::max<int64_t>((n + 4 * r - 1) / (4 * r), 1));
-    int64_t rows = (n + u - 1) / u;
-    rows = (rows + r - 1) / r * r;
-    *rows_per_unit = std::max<int64_t>(rows, r);
-    *units = std::max<int64_t>((n + *rows_per_unit - 1) / *rows_per_unit, 1);
+    const int64_t rows = (n + u - 1) / u, run = kRunSteps * r;
+    const int64_t parts = std::max<int64_t>((rows + run - 1) / run, 1);
+    BackwardPlan p{};
+    p.rows_per_unit = std::max(((rows + parts - 1) / parts + r - 1) / r * r, r);
+    const int64_t all = std::max<int64_t>((n + p.rows_per_unit - 1) / p.rows_per_unit, 1);
+    p.units = std::min(u, all);
+    p.passes = (all + p.units - 1) / p.units;
+    return p;
 }
 
 // Shared-memory opt-in of a kernel, once per device.
@@ -842,24 +868,42 @@ cudaError_t launch_rownorm(const RowNormArgs& a, cudaStream_t st) {
 }
 
 size_t rownorm_backward_workspace_bytes(int64_t n, int c, int nsamples) {
-    int64_t units = 0, rows = 0;
-    backward_units(n, c, nsamples, &units, &rows);
-    return static_cast<size_t>(units) * (SLAB_GATE + std::max(nsamples, 1)) * c * sizeof(float);
+    const BackwardPlan p = backward_plan(n, c, nsamples);
+    const size_t rows = SLAB_GATE + std::max(nsamples, 1);
+    return p.units * rows * c * sizeof(float) + (p.passes > 1 ? SLAB_GATE * c * sizeof(double) : 0);
 }
 
 cudaError_t launch_rownorm_backward(RowNormArgs a, const RowNormGrads& g, void* ws, cudaStream_t st) {
-    a.partial = static_cast<float*>(ws);
-    backward_units(a.n, a.c, a.nsamples, &a.units, &a.rows_per_unit);
+    const BackwardPlan p = backward_plan(a.n, a.c, a.nsamples);
     const int slab_rows = SLAB_GATE + (!a.gate ? 0 : (a.nsamples ? a.nsamples : 1));
-    if (a.n == 0) {
-        cudaError_t e = cudaMemsetAsync(ws, 0, static_cast<size_t>(a.units) * slab_rows * a.c * sizeof(float), st);
+    double* const totals = static_cast<double*>(ws);  // where there are several passes
+    a.partial = reinterpret_cast<float*>(totals + (p.passes > 1 ? SLAB_GATE * a.c : 0));
+    a.rows_per_unit = p.rows_per_unit;
+    const int64_t n = a.n, x_row = a.c * (a.x_dtype == DT_F32 ? 4 : 2), f_row = a.c * (a.f_dtype == DT_F32 ? 4 : 2);
+    auto advance = [](auto*& q, int64_t bytes) {
+        if (q) q = reinterpret_cast<std::remove_reference_t<decltype(q)>>(reinterpret_cast<uintptr_t>(q) + bytes);
+    };
+    for (int64_t pass = 0; pass < p.passes; ++pass) {
+        const int64_t row0 = pass * p.units * p.rows_per_unit;
+        RowNormArgs b = a;
+        b.n = std::min(p.units * p.rows_per_unit, n - row0);
+        b.units = std::max<int64_t>((b.n + p.rows_per_unit - 1) / p.rows_per_unit, 1);
+        advance(b.x, row0 * x_row), advance(b.dr, row0 * x_row), advance(b.dx, row0 * x_row);
+        advance(b.f, row0 * f_row), advance(b.dh, row0 * f_row), advance(b.df, row0 * f_row);
+        advance(b.coords, row0 * 16);
+        b.slab_clear = pass ? SLAB_GATE : slab_rows;
+        const cudaError_t e =
+            b.n ? launch_any(b, true, st)
+                : cudaMemsetAsync(a.partial, 0, static_cast<size_t>(b.units) * slab_rows * a.c * sizeof(float), st);
         if (e != cudaSuccess) return e;
+        const bool once = p.passes == 1, last = pass + 1 == p.passes;
+        slab_sum_kernel<<<dim3(a.c / 8, once ? slab_rows : SLAB_GATE), 1024, 0, st>>>(
+            a.partial, b.units, slab_rows, 0, a.c, totals, pass, last, g);
+        // the gate's rows of all the units there were
+        if (last && !once && slab_rows > SLAB_GATE)
+            slab_sum_kernel<<<dim3(a.c / 8, slab_rows - SLAB_GATE), 1024, 0, st>>>(a.partial, p.units, slab_rows, SLAB_GATE,
+                                                                                  a.c, totals, 0, true, g);
     }
-    if (a.n) {
-        cudaError_t e = launch_any(a, true, st);
-        if (e != cudaSuccess) return e;
-    }
-    slab_sum_kernel<<<dim3(a.c / 8, slab_rows), 1024, 0, st>>>(a.partial, a.units, slab_rows, a.c, g);
     return cudaGetLastError();
 }
 

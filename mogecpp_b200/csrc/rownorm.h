@@ -39,6 +39,7 @@ struct RowNormArgs {
     void* df;
     float* partial;  // [units][4 + gate rows][c]
     int64_t units, rows_per_unit;
+    int slab_clear;  // slab rows that start at zero (the others go on)
 };
 
 struct RowNormGrads {

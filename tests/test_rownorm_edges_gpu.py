@@ -94,3 +94,40 @@ def test_outputs_in_the_place_of_inputs(ex, n, c, x_dtype, f_dtype):
                                               ex._raw_stream()))
     ex.check()
     assert torch.equal(a, want["x"]) and torch.equal(b, want["f"])
+
+
+@pytest.mark.parametrize("spread", ["sorted", "shuffled", "one"])
+@pytest.mark.parametrize("n,c,nsamples", [(300000, 128, 32768), (200000, 64, 32768), (30000, 1024, 16000)])
+def test_long_runs_of_rows(ex, n, c, nsamples, spread):
+    """Many samples leave few units with long runs of rows.  Terms of one sign
+    whose every addition would round the same way (1/3 next to a large sum):
+    one fp32 chain over a unit's rows is off by up to 1e-3, runs of 1,024 steps
+    by (1024 + 16) 2^-24 of the sum at most (a term's own error, from the norm
+    of a constant gradient, adds 64 2^-24); a sample's gate is added up likewise,
+    one fp32 addition per change of sample besides."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    r = torch.randn(n, c, generator=gen, device="cuda")
+    third = torch.full((n, c), 1 / 3, device="cuda")
+    s = torch.randint(0, nsamples, (n,), generator=gen, device="cuda")
+    s = torch.sort(s).values if spread == "sorted" else (s if spread == "shuffled" else s * 0 + 5)
+    coords = torch.zeros(n, 4, dtype=torch.int32, device="cuda")
+    coords[:, 3] = s
+    one, zero = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    nrm = dict(kind="layer", w=one, b=one, eps=1e-6)
+    gate = torch.ones(nsamples, c, device="cuda")
+    got = ex.residual_norm_backward(r, torch.zeros_like(r), third, third, post=nrm, gate=gate, coords=coords,
+                                    pre=dict(nrm, b=zero))
+    ex.check()
+    t = third[0, 0].double().item()
+    rows = torch.bincount(s, minlength=nsamples).double()
+    u = 2.0 ** -24
+    limit = (1024 + 16 + 64) * u
+    for k in ("pre_b", "post_b"):
+        assert ((got[k].double() - n * t).abs() <= limit * n * t).all(), (k, ((got[k].double() / (n * t)) - 1).abs().max().item())
+    # f^ is zero, so that t is the post norm's bias, one
+    off = (got["gate"].double() - rows[:, None] * t).abs()
+    assert (off <= (limit + u * rows[:, None].clamp(max=1024)) * rows[:, None] * t + 1e-30).all()
+    hat, _ = norm64(r, nrm)
+    want, size = (t * hat).sum(0), (t * hat).abs().sum(0)
+    assert ((got["pre_w"].double() - want).abs() <= (limit + depth(c) * F32) * size).all()
+    torch.cuda.empty_cache()
