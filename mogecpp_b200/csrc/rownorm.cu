@@ -397,6 +397,8 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? (V > 1 ? 1 : 768 
                 if (has(v)) store8<FT>(a.h, row * a.c + (t + v * T) * 8, r + 4 * v);
         }
     }
+    // the copies past the last row have landed before the shared memory goes
+    cp_async_wait_all();
 }
 
 // Slab rows of a unit: pre_w, pre_b, post_w, post_b, then the gate's.
@@ -700,6 +702,8 @@ __global__ void __launch_bounds__(block_threads<T>(), T > 32 ? 512 / T : 2) rown
     };
     put(acc_pre_w, SLAB_PRE_W);
     put(acc_pre_b, SLAB_PRE_B);
+    // the copies past the run have landed before the shared memory goes
+    cp_async_wait_all();
 }
 
 // Column sums over the units, 8 columns (a 32-byte sector) a block, in double
@@ -760,8 +764,8 @@ int row_threads(int c) {
 // Units of the backward pass: enough to fill the GPU, at least four steps of
 // rows each where there are that many; but no more than 64 MiB of slabs, since
 // a gate per sample takes nsamples rows of each unit's.  Many samples therefore
-// leave fewer units, and the pass slows down: 400,000 x 128 bf16 takes 147 us
-// with 2 samples, 242 with 64, 1,015 with 512, 7,860 with 4,096 and 91,000 with
+// leave fewer units, and the pass slows down: 400,000 x 128 bf16 takes 144 us
+// with 2 samples, 239 with 64, 987 with 512, 7,750 with 4,096 and 90,500 with
 // 32,768.
 //
 // No unit's fp32 sums run over more than kRunSteps steps (an fp32 chain over
