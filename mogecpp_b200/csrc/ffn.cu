@@ -192,7 +192,9 @@ cudaError_t launch_gemm(const FfnGemmArgs& a, int ht, int cg, bool first, cudaSt
         if (cg == 2) return launch_gemm_t<MODE, 128, 2>(a, first, st);
         return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, first, st) : launch_gemm_t<MODE, 64, 1>(a, first, st);
     } else {
-        if (cg == 2) return ht == 256 ? launch_gemm_t<MODE, 256, 2>(a, first, st) : launch_gemm_t<MODE, 128, 2>(a, first, st);
+        if constexpr (MODE != FFN_DW)  // (its pairs have 256 columns, dw_plan)
+            if (cg == 2 && ht == 128) return launch_gemm_t<MODE, 128, 2>(a, first, st);
+        if (cg == 2) return launch_gemm_t<MODE, 256, 2>(a, first, st);
         if (ht == 256) return launch_gemm_t<MODE, 256, 1>(a, first, st);
         return ht == 128 ? launch_gemm_t<MODE, 128, 1>(a, first, st) : launch_gemm_t<MODE, 64, 1>(a, first, st);
     }

@@ -43,10 +43,6 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-
 // Shared-memory matrix descriptor, MN-major, 128-byte swizzle: the tile lies
 // as [group of 64 MN][k][64 MN x 16 bit], i.e. 128-byte rows along MN, 8-row
 // groups of k 1024 B apart (stride byte offset), groups of 64 MN
