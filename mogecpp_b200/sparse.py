@@ -469,24 +469,29 @@ class SparseCudaExecutor:
     def _ffn(self, ffn: dict, act: str, c: int, dtype):
         if act not in _ACT:
             raise L.MscError(L.MSC_E_INVALID, f"act must be one of {sorted(_ACT)}")
-        hidden, dt = ffn["w_gate"].shape[0], (dtype,)
-        return L.Ffn(_DT[dtype], hidden, _ACT[act], self._need(ffn["w_gate"], "w_gate", (hidden, c), dt),
-                     self._need(ffn["w_up"], "w_up", (hidden, c), dt),
-                     self._need(ffn["w_down"], "w_down", (c, hidden), dt),
+        gate = ffn.get("w_gate")
+        if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
+            raise L.MscError(L.MSC_E_INVALID, "w_gate must be a matrix")
+        hidden, dt = gate.shape[0], (dtype,)
+        return L.Ffn(_DT[dtype], hidden, _ACT[act], self._need(gate, "w_gate", (hidden, c), dt),
+                     self._need(ffn.get("w_up"), "w_up", (hidden, c), dt),
+                     self._need(ffn.get("w_down"), "w_down", (c, hidden), dt),
                      self._need_opt(ffn.get("b_gate"), "b_gate", (hidden,)),
                      self._need_opt(ffn.get("b_up"), "b_up", (hidden,)),
                      self._need_opt(ffn.get("b_down"), "b_down", (c,)))
 
     def _residual(self, n, c, x_dtype, f_dtype, post, gate, pre, res_scale, coords):
+        if f_dtype not in _DT:
+            raise L.MscError(L.MSC_E_INVALID, f"a branch of {f_dtype} is not supported")
+        samples = self._samples(gate, "gate", n, c, coords)
         return L.ResidualNormDesc(c, _DT[x_dtype], _DT[f_dtype], self._norm(post, "post", c), self._norm(pre, "pre", c),
-                                  None if gate is None else gate.data_ptr(),
-                                  self._samples(gate, "gate", n, c, coords), res_scale)
+                                  _ptr(gate), samples, res_scale)
 
     def _samples(self, gate, name, n, c, coords) -> int:
         """0 for a gate per channel, else the samples of a [nsamples, c] gate."""
         if gate is None:
             return 0
-        if gate.dim() == 1:
+        if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
             self._need(gate, name, (c,))
             return 0
         self._need(gate, name, (gate.shape[0], c))
@@ -596,9 +601,9 @@ class SparseCudaExecutor:
         arr = (L.FfnBlock * max(len(blocks), 1))()
         nsamples, hidden = 0, 8
         for i, b in enumerate(blocks):
-            dtype = b["ffn"]["w_gate"].dtype
+            dtype = getattr(b["ffn"].get("w_gate"), "dtype", None)
             if dtype not in _DT:
-                raise L.MscError(L.MSC_E_INVALID, f"feed-forward weights of {dtype} are not supported")
+                raise L.MscError(L.MSC_E_INVALID, f"feed-forward weights (w_gate) of {dtype} are not supported")
             ffn = self._ffn(b["ffn"], b.get("act", "silu"), c, dtype)
             gate = b.get("gate")
             ns = self._samples(gate, "gate", n, c, coords)

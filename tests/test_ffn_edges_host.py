@@ -48,3 +48,26 @@ def test_stack_workspace_covers_smaller_blocks(n, c):
     assert all(a <= b for a, b in zip(size, size[1:]))
     # no more than the splits' own rounding costs
     assert size[-1] <= 2 * most
+
+
+def test_wrong_arguments_are_refused_as_such(host_ex):
+    """Missing weights, weights and gates of another rank or kind, an unknown
+    branch type: the library's own error, before the library."""
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    f32 = x.float()
+    w, d = torch.zeros(128, 64, dtype=torch.bfloat16), torch.zeros(64, 128, dtype=torch.bfloat16)
+    ffn = dict(w_gate=w, w_up=w, w_down=d)
+    bad = [{**ffn, "w_gate": w[0]}, {**ffn, "w_down": None}, {"w_gate": w, "w_up": w}, {**ffn, "w_up": 1.0},
+           {**ffn, "w_gate": torch.zeros((), dtype=torch.bfloat16)}, {}]
+    for f in bad:
+        for call in (lambda: host_ex.gated_ffn(x, f), lambda: host_ex.gated_ffn_backward(x, x, f),
+                     lambda: host_ex.ffn_stack(f32, [dict(ffn=f)])):
+            with pytest.raises(L.MscError, match="w_"):
+                call()
+    for gate in (torch.zeros(()), torch.zeros(1, 1, 64), torch.zeros(8, 64).t(), 0.5):
+        with pytest.raises(L.MscError, match="gate"):
+            host_ex.residual_norm(f32, f32, gate=gate, coords=torch.zeros(4, 4, dtype=torch.int32))
+        with pytest.raises(L.MscError, match="gate"):
+            host_ex.residual_norm_backward(f32, f32, f32, None, gate=gate, coords=torch.zeros(4, 4, dtype=torch.int32))
+    with pytest.raises(L.MscError, match="branch"):
+        host_ex.residual_norm(f32, pre=dict(kind="rms"), branch_dtype=torch.float64)
