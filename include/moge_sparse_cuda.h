@@ -538,9 +538,11 @@ typedef struct {
 size_t msc_residual_norm_backward_workspace_bytes(int64_t n, int c, int nsamples);
 
 /* Backward pass of msc_residual_norm: r is the forward's output, dr and dh
- * the gradients of r and h (one of them may be NULL: zero).  The norms'
- * statistics are computed again from r and f.  Column sums are fp32 within a
- * run of rows and double across them, in a fixed order (no atomics). */
+ * the gradients of r and h.  dr may be NULL (zero); dh only without a pre norm
+ * (and not both).  The norms' statistics are computed again from r and f.
+ * Column sums are fp32 within a run of rows (at most 1,024 steps of a warp or
+ * block) and double across them, in a fixed order (no atomics).  With a gate
+ * per sample its time grows with nsamples beyond some ten. */
 int msc_residual_norm_backward(msc_ctx_t ctx, const msc_residual_norm_desc* desc, int64_t n, const void* r,
                                const void* f, const int32_t* coords, const void* dr, const void* dh,
                                const msc_residual_norm_grads* grads, void* ws, size_t ws_bytes, void* stream);
@@ -568,11 +570,13 @@ size_t msc_gated_ffn_workspace_bytes(int64_t n, int c, int hidden);
 
 /* Accumulation, activation and gating are fp32; the hidden values are
  * rounded once to the features' type (the tensor cores' operand; in fp16
- * they overflow beyond 65504, as any fp16 value).  y may be x. */
+ * they overflow beyond 65504, as any fp16 value) but in calls of up to 4, or
+ * 8, rows, which keep them fp32.  y may be x. */
 int msc_gated_ffn(msc_ctx_t ctx, const msc_ffn* ffn, int64_t n, int c, const void* x, void* y, void* ws,
                   size_t ws_bytes, void* stream);
 
-/* Gradients; NULL members are not written (the three weights together). */
+/* Gradients; NULL members are not written (the three weights together; one
+ * member at least, unless there are no rows). */
 typedef struct {
     void* dx;      /* [n][c]; neither x nor dy */
     void* w_gate;  /* as the weights, in their type */

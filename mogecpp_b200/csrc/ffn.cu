@@ -85,10 +85,10 @@ int k_splits(int64_t tiles, int ksteps, int* ksplit) {
 
 // No sum in one accumulator runs over more than 32768 elements: the tensor
 // core's fp32 accumulator truncates, so that a sum of one sign drifts towards
-// zero with the length of its chain.  Measured on dx (fp16, positive terms):
-// 2.6e-5 of the sum over 8,192 elements, 1.2e-4 over 32,768, 2.3e-4 over
-// 65,536, 4.4e-4 over 131,072, where the output's own rounding is 4.9e-4 at
-// most.
+// zero with the length of its chain.  Measured on dx (fp16, positive terms of
+// like size): 2.6e-5 of the sum over 4,096 elements, 1.2e-4 over 16,384, 2.2e-4
+// over 32,768 and 4.4e-4 over 65,536, where the output's own rounding is 4.9e-4
+// at most; a truncation of half 2^-23 per 8 elements fits them all.
 constexpr int kChainSteps = 512;
 void limit_chain(int ksteps, int* splits, int* ksplit) {
     if (*ksplit <= kChainSteps) return;

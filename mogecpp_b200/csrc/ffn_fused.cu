@@ -9,8 +9,9 @@
 //   h = act(D_g + bg) * (D_u + bu)  (epilogue warps -> shared memory, 16 bits)
 //   Y += h Wd[:, chunk]^T           (TMEM, 128 rows x c columns, K = 64)
 // The weights stream through shared memory once per 256 rows (they stay in
-// L2).  The epilogue is the long pole (a gated activation an element, bound by
-// the special-function unit and its own hand-overs), so that its warps take D
+// L2).  The epilogue is the long pole (a gated activation an element: issue
+// slots 57 % busy and the special-function unit 48 % at 128 channels, 60 and 30 %
+// at 64, the rest is its hand-overs), so that its warps take D
 // into registers and release it before they are done computing, and the next
 // chunk's D is there when they come back.  The two products have an issuing
 // warp each, so that neither waits for the other's operands.
@@ -21,15 +22,16 @@
 // against 170 at 402,131 x 128 -> 512, bf16), each subtile has a group.
 //
 // Y's chain in its accumulator is the whole hidden size, at most 65,536: not
-// cut at 32,768 as the products of ffn.cu are, since what it then drifts by for
-// terms of one sign stays below half of fp16's rounding.
+// cut at 32,768 as the products of ffn.cu are (it would have to leave the SM):
+// what the longest drifts by for terms of one sign, 4.4e-4 there, stays below
+// fp16's own rounding.
 //
 // TMEM: Y 2 x 128 columns, D 2 x 128 columns.  Warps: 0 TMA producer, 1 and 2
 // MMA issuers (D, Y), 3 TMEM allocation (and stores), 4 on epilogue (8 per
 // group: lane quarter x half of the chunk).  Every wait is bounded, as in
 // ffn_gemm.cuh.
 //
-// Measured: 402,131 x 128 -> 512 bf16 170 us (0.93 PFLOP/s; two kernels with
+// Measured: 402,131 x 128 -> 512 bf16 172 us (0.92 PFLOP/s; two kernels with
 // h in memory: 291 us); without the activations the products and copies alone
 // take 120 us, bound by shared-memory operand reads of 128-column products
 // and the weights' way from L2 (24 KB per item and SM).  101,117 x 64 -> 256

@@ -27,8 +27,10 @@
 // steps deep.  Measured at 402,131 x 128 bf16 with a gate per sample: forward
 // 178 us as first written, 101 with packed arithmetic and the gate folded into
 // the post norm, 90 with unpredicated loads, 73.5 with the ring (5.7 TB/s, 87 %
-// of the copy rate); backward 255, 206, 164 and 131 us (4.8 TB/s; bound by
-// instruction issue at the 16 warps that 128 registers allow).
+// of the copy rate); backward 255, 206, 164 and 128 us (4.9 TB/s; issue slots
+// 63 %: the row sums' shuffles at the 16 warps that 128 registers allow).
+// Above 2048 channels the backward pass spills (436 to 564 bytes a thread):
+// 20,000 x 4096 bf16 takes 1,026 us, x 8192 954, x 2048 171.
 //
 // The backward column sums are kept in fp32 registers over a unit's (warp's
 // or block's) run of rows, at most 1,024 steps, written once per unit, and

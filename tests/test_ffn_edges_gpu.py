@@ -131,12 +131,13 @@ def test_stack_of_mixed_hidden_sizes(ex, n, c, sizes):
 # pass of that many rows and few channels is one kernel, whose chain is the whole hidden size)
 @pytest.mark.parametrize("n,c", [(9500, 1024), (4900, 512), (20000, 128)])
 def test_long_sums_do_not_drift(ex, n, c):
-    """65,536 hidden units, terms of one sign.  A chain of 32,768 elements in
-    one fp32 accumulator drifts by 1.2e-4 of its sum (measured: the tensor core
-    truncates), one of 131,072 (dx in one accumulator) by 4.4e-4; the parts'
-    fp32 additions add 4 2^-24.  The mean over 64 x c outputs takes their 16-bit
-    rounding out (2^-11 / sqrt(3 * 64 c) < 4e-6).  Limit: twice the short
-    chain's drift; the single kernel's chain of 65,536, twice that."""
+    """65,536 hidden units, terms of one sign.  The tensor core truncates its
+    fp32 accumulator: a step of 8 elements loses up to 2^-23 of the sum so far,
+    which averages half of the total, so that a chain of 32,768 drifts by
+    32768 / 8 * 2^-23 / 2 = 2.4e-4 at most, and one of 65,536 (y in the single
+    kernel; before the limit also dx, whose dg half of the chain is small here)
+    by 4.9e-4.  The mean over 64 x c outputs takes their 16-bit rounding out
+    (2^-11 / sqrt(3 * 64 c) < 4e-6)."""
     hidden = 65536
     gen = torch.Generator(device="cuda").manual_seed(n)
 
